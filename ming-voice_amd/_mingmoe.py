@@ -44,6 +44,20 @@ class Experts(ctypes.Structure):
                 ("sgu_stride_e", _I64), ("sd_stride_e", _I64), ("w_gu_slabs", _P), ("w_d_slabs", _P)]
 
 
+class Pages(ctypes.Structure):
+    """mm_pages: a pool of cache pages, k [n_pages, nkv, page, dqk] and v [n_pages, nkv, page, dv] with their strides."""
+    _fields_ = [("k", _P), ("v", _P), ("dtype", ctypes.c_int32), ("nkv", ctypes.c_int32), ("dqk", ctypes.c_int32),
+                ("dv", ctypes.c_int32), ("n_pages", _I64), ("page", _I64), ("k_page_stride", _I64),
+                ("k_head_stride", _I64), ("k_row_stride", _I64), ("v_page_stride", _I64), ("v_head_stride", _I64),
+                ("v_row_stride", _I64)]
+
+
+class Batch(ctypes.Structure):
+    """mm_batch: packed tokens of several streams (cu, kv_lens and the page table, device arrays of one dtype)."""
+    _fields_ = [("cu", _P), ("kv_lens", _P), ("table", _P), ("table_stride", _I64), ("max_pages", _I64),
+                ("seqs", _I64), ("tokens", _I64), ("idx_dtype", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "mm_version": ([], ctypes.c_int),
     "mm_last_error": ([ctypes.c_char_p, ctypes.c_size_t], ctypes.c_size_t),
@@ -102,6 +116,20 @@ SIGNATURES = {
     "mm_down_slabs": ([ctypes.POINTER(Experts), _P, _P], ctypes.c_int),
 }
 
+# the entry points of include/mingpaged.h
+PAGED_VERSION = 1
+PAGED_SIGNATURES = {
+    "mm_paged_version": ([], ctypes.c_int),
+    "mm_paged_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, ctypes.POINTER(Pages),
+                         ctypes.POINTER(Batch), _P, _I64, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P], ctypes.c_int),
+    "mm_paged_attn_workspace": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
+    "mm_paged_attn": ([_P, _I64, _I64, _I32, ctypes.POINTER(Pages), ctypes.POINTER(Batch), _F32, _P, _I64, _I64, _P,
+                       _I64, _P], ctypes.c_int),
+    "mm_prompt_attn_workspace": ([_I64, _I64, _I32, _I32, _I32, _I32], _I64),
+    "mm_prompt_attn": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64,
+                        _I64, _F32, _P, _I64, _I64, _P, _I64, _P], ctypes.c_int),
+}
+
 _lib = None
 
 
@@ -114,13 +142,17 @@ def load(path=LIB_PATH):
         raise RuntimeError(f"libmingmoe.so not found at {path}: build it with `python build_lib.py` "
                            "(or __graft_entry__.build()); there is no fallback path")
     lib = ctypes.CDLL(path)
-    for name, (args, res) in SIGNATURES.items():
-        fn = getattr(lib, name)
+    for name, (args, res) in {**SIGNATURES, **PAGED_SIGNATURES}.items():
+        fn = getattr(lib, name, None)
+        if fn is None:
+            raise RuntimeError(f"libmingmoe.so has no {name}: rebuild it")
         fn.argtypes = args
         fn.restype = res
     v = lib.mm_version()
     if v != ABI_VERSION:
         raise RuntimeError(f"libmingmoe.so ABI version {v}, expected {ABI_VERSION}: rebuild it")
+    if (v := lib.mm_paged_version()) != PAGED_VERSION:
+        raise RuntimeError(f"libmingmoe.so paged version {v}, expected {PAGED_VERSION}: rebuild it")
     _lib = lib
     return lib
 

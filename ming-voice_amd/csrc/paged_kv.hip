@@ -1,0 +1,514 @@
+// The paged cache of several streams: the append of new tokens with their rotation, the attention of new tokens over the
+// pages, and the attention over packed prompts (C ABI: mingpaged.h).
+//
+//   paged_append_kernel   rotation and stores, one pass over q, k and v
+//   attn_rows_kernel      attention, one wave per token and query head
+#include <cmath>
+
+#include "mingpaged.h"
+#include "mm_common.h"
+
+namespace {
+
+using namespace mmd;
+
+// ------------------------------------------------------------------------------------------ shared pieces
+
+// n / d for n < 2^31 by a multiplication: m = floor(2^(31 + l) / d) + 1 with l = ceil(log2 d) exceeds 2^(31 + l) / d by at
+// most 1 <= 2^l / d, so the product is off by less than 1 / d for every such n.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+};
+
+FastDiv fast_div(int64_t d) {
+  FastDiv f{static_cast<uint32_t>(d), 0, 0};
+  if (d > 1) {
+    int l = 0;
+    while ((1LL << l) < d) ++l;
+    f.m = static_cast<uint32_t>((1ULL << (31 + l)) / static_cast<uint64_t>(d) + 1);
+    f.s = l - 1;
+  }
+  return f;
+}
+
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return f.d == 1 ? n : __umulhi(n, f.m) >> f.s;
+}
+
+// The batch as the kernels see it: device arrays of one index type, every value clamped before use, so that no content of
+// them leads outside a buffer.
+struct Batch {
+  const void* cu;
+  const void* lens;
+  const void* table;
+  int64_t table_stride;
+  int i64;          // the arrays hold 64-bit numbers
+  int seqs, tokens;
+  int max_keys;     // max_pages * page
+};
+
+__device__ __forceinline__ int64_t idx_at(const void* p, int i64, int64_t i) {
+  return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// A stream's first token, the number of its tokens and the rows of its cache that count (-1: outside the table).
+struct Stream {
+  int first, n, kv;
+};
+
+__device__ __forceinline__ Stream stream_at(const Batch& a, int b) {
+  const int64_t c0 = idx_at(a.cu, a.i64, b), c1 = idx_at(a.cu, a.i64, b + 1);
+  Stream s;
+  s.first = static_cast<int>(min(max(c0, static_cast<int64_t>(0)), static_cast<int64_t>(a.tokens)));
+  s.n = static_cast<int>(min(max(c1, static_cast<int64_t>(s.first)), static_cast<int64_t>(a.tokens))) - s.first;
+  if (a.lens) {
+    const int64_t kv = idx_at(a.lens, a.i64, b);
+    s.kv = kv < 0 || kv > a.max_keys ? -1 : static_cast<int>(kv);
+  } else {
+    s.kv = s.n;  // a prompt's own rows
+  }
+  return s;
+}
+
+// The stream that token t belongs to (seqs: none), found by the whole wave: the number of streams that end at or before t.
+__device__ __forceinline__ int stream_of_token(const Batch& a, int t) {
+  int b = 0;
+  for (int base = 0; base < a.seqs; base += kWave) {
+    const int i = base + lane_id();
+    const bool before = i < a.seqs && idx_at(a.cu, a.i64, min(i, a.seqs - 1) + 1) <= t;
+    const int n = __popcll(__ballot(before));
+    b += n;
+    if (n < kWave) break;
+  }
+  return min(b, a.seqs);
+}
+
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::kBf16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      x[2 * i] = f16_to_f32(static_cast<uint16_t>(w[i]));
+      x[2 * i + 1] = f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (T::kBf16) return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
+  else return static_cast<uint32_t>(f32_to_f16(lo)) | (static_cast<uint32_t>(f32_to_f16(hi)) << 16);
+}
+
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+}
+
+__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void st16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// Rows [tokens, heads, d] of a packed tensor, or one page's: element strides.
+struct Rows {
+  uint16_t* p;
+  int64_t ts, hs;
+  __device__ __forceinline__ uint16_t* at(int64_t t, int h) const { return p + t * ts + h * hs; }
+};
+
+struct Pool {
+  uint16_t* p;
+  int64_t ps, hs, rs;
+  __device__ __forceinline__ uint16_t* at(int64_t page, int h, int row) const { return p + page * ps + h * hs + row * rs; }
+};
+
+// ------------------------------------------------------------------------------------------ append
+
+struct AppendArgs {
+  Rows q, k, v, q_out, k_out;  // k_out.p NULL: not wanted
+  Pool kp, vp;
+  Batch batch;
+  FastDiv page, iph;  // iph: items of a q or k head
+  int64_t n_pages;
+  const float* inv_freq;
+  int nh, nkv, dqk, dv, pairs, rot_offset, interleaved;
+  int q_in_place, k_in_place;  // the dims that do not turn are there already
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxPairs = 128;
+
+// A workgroup takes TPW tokens. Each of its waves finds the streams, positions and page rows of its tokens; then the angles
+// of all pairs are turned into cosines and sines once for all heads; then the items (16 elements of a head that turn, or 8
+// that only move) go through the threads.
+template <class T, int TPW>
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
+  __shared__ int s_pos[TPW], s_row[TPW];
+  __shared__ int64_t s_page[TPW];  // -1: the token is not stored
+  __shared__ float s_cos[TPW * kMaxPairs], s_sin[TPW * kMaxPairs];
+  const int tid = threadIdx.x, wave = tid / kWave;
+  const int t0 = static_cast<int>(blockIdx.x) * TPW;
+  for (int j = wave; j < TPW; j += kAppendThreads / kWave) {
+    const int t = t0 + j;
+    int pos = 0, row = 0;
+    int64_t page = -2;  // no stream owns the token: nothing of it is written
+    if (t < a.batch.tokens) {
+      const int b = stream_of_token(a.batch, t);
+      if (b < a.batch.seqs) {
+        const Stream s = stream_at(a.batch, b);
+        page = -1;
+        pos = s.kv < 0 ? 0 : s.kv - s.n + (t - s.first);
+        if (s.kv >= 0 && pos >= 0 && pos < a.batch.max_keys) {
+          const int pg = static_cast<int>(div_by(pos, a.page));
+          const int64_t id = idx_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + pg);
+          row = pos - pg * static_cast<int>(a.page.d);
+          if (id >= 0 && id < a.n_pages) page = id;
+        }
+      }
+    }
+    if (lane_id() == 0) {
+      s_pos[j] = pos;
+      s_row[j] = row;
+      s_page[j] = page;
+    }
+  }
+  __syncthreads();
+  // angles in 64 bits, reduced to [-1/2, 1/2] turns: a position of 10^6 leaves 2^-33 of a turn, where 32 bits would leave
+  // a hundredth of a turn
+  for (int i = tid; i < TPW * a.pairs; i += kAppendThreads) {
+    const int j = i / a.pairs, p = i - j * a.pairs;
+    const double turns = static_cast<double>(s_pos[j]) * static_cast<double>(a.inv_freq[p]) * 0.15915494309189533577;
+    float s, c;
+    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+    s_cos[j * kMaxPairs + p] = c;
+    s_sin[j * kMaxPairs + p] = s;
+  }
+  __syncthreads();
+  const int rot_items = a.pairs / 8, heads = a.nh + a.nkv;
+  const int qk_items = heads * static_cast<int>(a.iph.d), vc = a.dv / 8, items = qk_items + a.nkv * vc;
+  for (int i = tid; i < TPW * items; i += kAppendThreads) {
+    const int j = TPW == 1 ? 0 : i / items, it = i - j * items, t = t0 + j;
+    const int64_t page = s_page[j];
+    if (page == -2) continue;
+    const int row = s_row[j];
+    if (it >= qk_items) {
+      const int h = (it - qk_items) / vc, c = (it - qk_items) - h * vc;
+      if (page >= 0) st16(a.vp.at(page, h, row) + 8 * c, ld16(a.v.at(t, h) + 8 * c));
+      continue;
+    }
+    const int head = static_cast<int>(div_by(it, a.iph)), c = it - head * static_cast<int>(a.iph.d);
+    const bool isq = head < a.nh;
+    const int h = isq ? head : head - a.nh;
+    const uint16_t* src = isq ? a.q.at(t, h) : a.k.at(t, h);
+    uint16_t* dst = isq ? a.q_out.at(t, h) : a.k_out.p ? a.k_out.at(t, h) : nullptr;
+    uint16_t* pool = !isq && page >= 0 ? a.kp.at(page, h, row) : nullptr;
+    if (c >= rot_items) {  // a chunk that does not turn
+      const int ch = c - rot_items, d = ch < a.rot_offset / 8 ? 8 * ch : 8 * ch + 2 * a.pairs;
+      const bool stays = isq ? a.q_in_place : a.k_in_place;
+      if (stays && !pool) continue;
+      const uint4 x = ld16(src + d);
+      if (dst && !stays) st16(dst + d, x);
+      if (pool) st16(pool + d, x);
+      continue;
+    }
+    const int d0 = a.rot_offset + (a.interleaved ? 16 * c : 8 * c), d1 = a.interleaved ? d0 + 8 : d0 + a.pairs;
+    float x0[8], x1[8], y0[8], y1[8];
+    unpack8<T>(ld16(src + d0), x0);
+    unpack8<T>(ld16(src + d1), x1);
+    const float* cs = s_cos + j * kMaxPairs + 8 * c;
+    const float* sn = s_sin + j * kMaxPairs + 8 * c;
+    if (a.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y0[2 * e] = fmaf(x0[2 * e], cs[e], -x0[2 * e + 1] * sn[e]);
+        y0[2 * e + 1] = fmaf(x0[2 * e + 1], cs[e], x0[2 * e] * sn[e]);
+        y1[2 * e] = fmaf(x1[2 * e], cs[4 + e], -x1[2 * e + 1] * sn[4 + e]);
+        y1[2 * e + 1] = fmaf(x1[2 * e + 1], cs[4 + e], x1[2 * e] * sn[4 + e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y0[e] = fmaf(x0[e], cs[e], -x1[e] * sn[e]);
+        y1[e] = fmaf(x1[e], cs[e], x0[e] * sn[e]);
+      }
+    }
+    const uint4 w0 = pack8<T>(y0), w1 = pack8<T>(y1);
+    if (dst) {
+      st16(dst + d0, w0);
+      st16(dst + d1, w1);
+    }
+    if (pool) {
+      st16(pool + d0, w0);
+      st16(pool + d1, w1);
+    }
+  }
+}
+
+template <class T>
+int launch_append(const AppendArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((paged_append_kernel<T, 1>), dim3(static_cast<unsigned>(a.batch.tokens)), dim3(kAppendThreads), 0, st, a);
+  return mm::check_launch("paged_append");
+}
+
+// ------------------------------------------------------------------------------------------ attention
+
+struct AttnArgs {
+  Rows q, out;
+  Rows k, v;    // a prompt's packed rows
+  Pool kp, vp;  // the cache
+  Batch batch;
+  FastDiv page, group;
+  int64_t n_pages;
+  int nh, nkv, dqk, dv;
+  float scale;
+};
+
+// One wave per token and query head: 64 keys at a time, a key to a lane for the scores, dims to the lanes for the values.
+template <class T, bool PAGED>
+__global__ __launch_bounds__(kWave) void attn_rows_kernel(AttnArgs a) {
+  __shared__ float s_q[256], s_p[kWave];
+  __shared__ const uint16_t* s_v[kWave];
+  const int t = blockIdx.x, h = blockIdx.y, lane = lane_id();
+  const int b = stream_of_token(a.batch, t);
+  if (b >= a.batch.seqs) return;
+  const Stream s = stream_at(a.batch, b);
+  uint16_t* o = a.out.at(t, h);
+  if (s.kv < 0) {
+    for (int d = lane; d < a.dv; d += kWave) T::st(o, d, NAN);
+    return;
+  }
+  const int kvh = static_cast<int>(div_by(h, a.group)), lim = s.kv - s.n + (t - s.first) + 1;
+  for (int d = lane; d < a.dqk; d += kWave) s_q[d] = T::ld(a.q.at(t, h), d);
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < lim; k0 += kWave) {
+    const int key = k0 + lane;
+    const uint16_t *kr = nullptr, *vr = nullptr;
+    if (key < lim) {
+      if constexpr (PAGED) {
+        const int pg = static_cast<int>(div_by(key, a.page)), row = key - pg * static_cast<int>(a.page.d);
+        const int64_t id = idx_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + pg);
+        if (id >= 0 && id < a.n_pages) {
+          kr = a.kp.at(id, kvh, row);
+          vr = a.vp.at(id, kvh, row);
+        }
+      } else {
+        kr = a.k.at(s.first + key, kvh);
+        vr = a.v.at(s.first + key, kvh);
+      }
+    }
+    float sc = 0.f;
+    if (kr)
+      for (int d = 0; d < a.dqk; d += 8) {
+        float x[8];
+        unpack8<T>(ld16(kr + d), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc = fmaf(x[e], s_q[d + e], sc);
+      }
+    sc = kr ? sc * a.scale : -INFINITY;
+    const float mn = fmaxf(m, wave_max(sc)), mu = mn == -INFINITY ? 0.f : mn;
+    const float p = kr ? expf(sc - mu) : 0.f, alpha = expf(m - mu);
+    m = mn;
+    l = fmaf(l, alpha, wave_sum(p));
+    __syncthreads();
+    s_p[lane] = p;
+    s_v[lane] = vr;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+    for (int j = 0; j < kWave; ++j) {
+      if (!s_v[j]) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = lane + kWave * e;
+        if (d < a.dv) acc[e] = fmaf(s_p[j], T::ld(s_v[j], d), acc[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = lane + kWave * e;
+    if (d < a.dv) T::st(o, d, m == -INFINITY ? 0.f : acc[e] / l);
+  }
+}
+
+template <class T, bool PAGED>
+int launch_attn(const AttnArgs& a, hipStream_t st, const char* what) {
+  hipLaunchKernelGGL((attn_rows_kernel<T, PAGED>), dim3(static_cast<unsigned>(a.batch.tokens), static_cast<unsigned>(a.nh)),
+                     dim3(kWave), 0, st, a);
+  return mm::check_launch(what);
+}
+
+// ------------------------------------------------------------------------------------------ checks on the host
+
+constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxKeys = (1LL << 31) - 1;
+
+int check_rows(const char* what, const char* name, const void* p, int64_t ts, int64_t hs, int align) {
+  MM_REQUIRE(p, "%s: null %s", what, name);
+  MM_REQUIRE((reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(align - 1)) == 0, "%s: %s must be %d-byte aligned",
+             what, name, align);
+  MM_REQUIRE(ts >= 0 && hs >= 0 && ts % (align / 2) == 0 && hs % (align / 2) == 0,
+             "%s: strides of %s must keep rows %d-byte aligned", what, name, align);
+  return MM_OK;
+}
+
+int check_shape(const char* what, int dtype, int nh, int nkv, int dqk, int dv) {
+  MM_REQUIRE(dtype == MM_BF16 || dtype == MM_FP16, "%s: bf16 or fp16 tensors", what);
+  MM_REQUIRE(nh >= 1 && nkv >= 1 && nh <= 4096 && nh % nkv == 0, "%s: nh=%d must be a multiple of nkv=%d, at most 4096",
+             what, nh, nkv);
+  MM_REQUIRE(dqk >= 8 && dqk <= 256 && dqk % 8 == 0, "%s: dqk=%d must be a multiple of 8 up to 256", what, dqk);
+  MM_REQUIRE(dv >= 8 && dv <= 256 && dv % 8 == 0, "%s: dv=%d must be a multiple of 8 up to 256", what, dv);
+  return MM_OK;
+}
+
+int check_tokens(const char* what, int64_t tokens, int64_t seqs) {
+  MM_REQUIRE(tokens >= 0 && tokens <= kMaxTokens, "%s: bad number of tokens %lld", what, (long long)tokens);
+  MM_REQUIRE(seqs >= 0 && seqs <= kMaxSeqs, "%s: bad number of streams %lld", what, (long long)seqs);
+  return MM_OK;
+}
+
+int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) {
+  MM_REQUIRE(g && b, "%s: null descriptor", what);
+  int rc = check_shape(what, g->dtype, nh, g->nkv, g->dqk, g->dv);
+  if (rc) return rc;
+  if ((rc = check_tokens(what, b->tokens, b->seqs))) return rc;
+  MM_REQUIRE(b->idx_dtype == MM_INT32 || b->idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
+  MM_REQUIRE(g->page >= 1 && g->n_pages >= 0 && b->max_pages >= 0 && b->table_stride >= 0, "%s: bad page or table sizes", what);
+  MM_REQUIRE(b->max_pages <= kMaxKeys / g->page, "%s: max_pages * page must be below 2^31", what);
+  MM_REQUIRE(b->cu && b->kv_lens && (b->table || b->max_pages == 0), "%s: null batch array", what);
+  MM_REQUIRE(g->n_pages == 0 || (g->k && g->v), "%s: null pool", what);
+  MM_REQUIRE(mm::aligned16(g->k) && mm::aligned16(g->v), "%s: the pool must be 16-byte aligned", what);
+  const int64_t st[6] = {g->k_page_stride, g->k_head_stride, g->k_row_stride, g->v_page_stride, g->v_head_stride, g->v_row_stride};
+  for (int64_t s : st) MM_REQUIRE(s >= 0 && s % 8 == 0, "%s: the pool's strides must be multiples of 8", what);
+  return MM_OK;
+}
+
+Batch batch_of(const mm_pages* g, const mm_batch* b) {
+  return Batch{b->cu, b->kv_lens, b->table, b->table_stride, b->idx_dtype == MM_INT64, static_cast<int>(b->seqs),
+               static_cast<int>(b->tokens), static_cast<int>(b->max_pages * g->page)};
+}
+
+Rows rows_of(const void* p, int64_t ts, int64_t hs) { return Rows{static_cast<uint16_t*>(const_cast<void*>(p)), ts, hs}; }
+
+void set_pool(const mm_pages* g, Pool& k, Pool& v) {
+  k = Pool{static_cast<uint16_t*>(g->k), g->k_page_stride, g->k_head_stride, g->k_row_stride};
+  v = Pool{static_cast<uint16_t*>(g->v), g->v_page_stride, g->v_head_stride, g->v_row_stride};
+}
+
+}  // namespace
+
+extern "C" int mm_paged_version(void) { return MM_PAGED_VERSION; }
+
+extern "C" int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                               const void* v, int64_t v_ts, int64_t v_hs, int nh, const mm_pages* pages,
+                               const mm_batch* batch, const float* inv_freq, int64_t pairs, int rot_offset, int interleaved,
+                               void* q_out, int64_t qo_ts, int64_t qo_hs, void* k_out, int64_t ko_ts, int64_t ko_hs,
+                               void* stream) {
+  const char* what = "paged_append";
+  int rc = check_paged(what, nh, pages, batch);
+  if (rc) return rc;
+  if (!inv_freq) pairs = rot_offset = 0;
+  MM_REQUIRE(pairs >= 0 && pairs % 8 == 0 && rot_offset >= 0 && rot_offset % 8 == 0 && pairs <= kMaxPairs &&
+                 rot_offset + 2 * pairs <= pages->dqk,
+             "paged_append: %lld pairs from dim %d on do not fit a head of %d (multiples of 8)", (long long)pairs, rot_offset,
+             pages->dqk);
+  if (batch->tokens == 0 || batch->seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "k", k, k_ts, k_hs, 16)) ||
+      (rc = check_rows(what, "v", v, v_ts, v_hs, 16)) || (rc = check_rows(what, "q_out", q_out, qo_ts, qo_hs, 16)))
+    return rc;
+  if (k_out && (rc = check_rows(what, "k_out", k_out, ko_ts, ko_hs, 16))) return rc;
+  AppendArgs a{};
+  a.q = rows_of(q, q_ts, q_hs);
+  a.k = rows_of(k, k_ts, k_hs);
+  a.v = rows_of(v, v_ts, v_hs);
+  a.q_out = rows_of(q_out, qo_ts, qo_hs);
+  a.k_out = rows_of(k_out, ko_ts, ko_hs);
+  set_pool(pages, a.kp, a.vp);
+  a.batch = batch_of(pages, batch);
+  a.page = fast_div(pages->page);
+  a.n_pages = pages->n_pages;
+  a.inv_freq = inv_freq;
+  a.nh = nh;
+  a.nkv = pages->nkv;
+  a.dqk = pages->dqk;
+  a.dv = pages->dv;
+  a.pairs = static_cast<int>(pairs);
+  a.rot_offset = rot_offset;
+  a.interleaved = interleaved != 0;
+  a.iph = fast_div(a.pairs / 8 + (a.dqk - 2 * a.pairs) / 8);
+  a.q_in_place = q_out == q && qo_ts == q_ts && qo_hs == q_hs;
+  a.k_in_place = k_out == nullptr || (k_out == k && ko_ts == k_ts && ko_hs == k_hs);
+  return pages->dtype == MM_BF16 ? launch_append<BF16>(a, MM_STREAM(stream)) : launch_append<FP16>(a, MM_STREAM(stream));
+}
+
+extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+  if (check_shape("paged_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("paged_attn", tokens, seqs) || max_keys < 0 ||
+      max_keys > kMaxKeys)
+    return -1;
+  return 0;
+}
+
+extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
+                             float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  const char* what = "paged_attn";
+  int rc = check_paged(what, nh, pages, batch);
+  if (rc) return rc;
+  if (batch->tokens == 0 || batch->seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "out", out, o_ts, o_hs, 8))) return rc;
+  AttnArgs a{};
+  a.q = rows_of(q, q_ts, q_hs);
+  a.out = rows_of(out, o_ts, o_hs);
+  set_pool(pages, a.kp, a.vp);
+  a.batch = batch_of(pages, batch);
+  a.page = fast_div(pages->page);
+  a.group = fast_div(nh / pages->nkv);
+  a.n_pages = pages->n_pages;
+  a.nh = nh;
+  a.nkv = pages->nkv;
+  a.dqk = pages->dqk;
+  a.dv = pages->dv;
+  a.scale = scale;
+  return pages->dtype == MM_BF16 ? launch_attn<BF16, true>(a, MM_STREAM(stream), what)
+                                 : launch_attn<FP16, true>(a, MM_STREAM(stream), what);
+}
+
+extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv) {
+  if (check_shape("prompt_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("prompt_attn", tokens, seqs)) return -1;
+  return 0;
+}
+
+extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                              const void* v, int64_t v_ts, int64_t v_hs, int dtype, int nh, int nkv, int dqk, int dv,
+                              const void* cu, int idx_dtype, int64_t seqs, int64_t tokens, float scale, void* out,
+                              int64_t o_ts, int64_t o_hs, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "prompt_attn";
+  int rc = check_shape(what, dtype, nh, nkv, dqk, dv);
+  if (rc) return rc;
+  if ((rc = check_tokens(what, tokens, seqs))) return rc;
+  MM_REQUIRE(idx_dtype == MM_INT32 || idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
+  MM_REQUIRE(cu, "%s: null cu", what);
+  if (tokens == 0 || seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "k", k, k_ts, k_hs, 16)) ||
+      (rc = check_rows(what, "v", v, v_ts, v_hs, 16)) || (rc = check_rows(what, "out", out, o_ts, o_hs, 8)))
+    return rc;
+  AttnArgs a{};
+  a.q = rows_of(q, q_ts, q_hs);
+  a.k = rows_of(k, k_ts, k_hs);
+  a.v = rows_of(v, v_ts, v_hs);
+  a.out = rows_of(out, o_ts, o_hs);
+  a.batch = Batch{cu, nullptr, nullptr, 0, idx_dtype == MM_INT64, static_cast<int>(seqs), static_cast<int>(tokens), 0};
+  a.page = fast_div(1);
+  a.group = fast_div(nh / nkv);
+  a.nh = nh;
+  a.nkv = nkv;
+  a.dqk = dqk;
+  a.dv = dv;
+  a.scale = scale;
+  return dtype == MM_BF16 ? launch_attn<BF16, false>(a, MM_STREAM(stream), what)
+                          : launch_attn<FP16, false>(a, MM_STREAM(stream), what);
+}

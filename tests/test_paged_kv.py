@@ -1,0 +1,261 @@
+"""CPU checks of the paged cache: the header and its structs, the refusals of the C entries and of the wrappers, the
+arithmetic that turns positions into pages, and the oracle against torch's own attention."""
+import ctypes
+import hashlib
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import _mingmoe as mm
+import paged_kv as PK
+from oracle import paged_oracle as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "mingpaged.h")
+BF = torch.bfloat16
+
+
+def _text():
+    return re.sub(r"/\*.*?\*/", " ", open(HEADER).read(), flags=re.S)
+
+
+def test_header_declares_the_entry_points_and_the_library_exports_them():
+    names = sorted(set(re.findall(r"^\s*(?:int|int64_t)\s+(mm_\w+)\s*\(", _text(), re.M)))
+    assert names == sorted(mm.PAGED_SIGNATURES)
+    lib = mm.load()
+    assert all(hasattr(lib, n) for n in names)
+    assert lib.mm_paged_version() == mm.PAGED_VERSION
+
+
+# digests of the header's interface (no comments) by version, as tests/test_abi.py keeps them for mingmoe.h
+INTERFACES = {1: "d5929419b43b0513"}
+
+
+def test_the_version_moves_with_the_interface():
+    text = _text()
+    version = int(re.search(r"#define MM_PAGED_VERSION (\d+)", text).group(1))
+    code = " ".join(re.sub(r"#define MM_PAGED_VERSION \d+", "", text).split())
+    assert hashlib.sha256(code.encode()).hexdigest()[:16] == INTERFACES[version]
+    assert version == mm.PAGED_VERSION == max(INTERFACES)
+
+
+@pytest.mark.parametrize("name,struct", [("mm_pages", mm.Pages), ("mm_batch", mm.Batch)])
+def test_struct_layout_matches_c(tmp_path, name, struct):
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "mingpaged.h"\n'
+                   f'int main(void){{printf("%zu", sizeof({name}));'
+                   + "".join(f'printf(" %zu", offsetof({name}, {f}));' for f, _ in struct._fields_) + 'return 0;}\n')
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.dirname(HEADER), str(src), "-o", str(exe)], check=True)
+    vals = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert vals == [ctypes.sizeof(struct)] + [getattr(struct, f).offset for f, _ in struct._fields_]
+
+
+# ------------------------------------------------------------------------------------------------ refusals, C entries
+
+P = 4096  # an aligned address that no refused call reads
+
+
+def pages(**kw):
+    g = mm.Pages(P, P, mm.MM_BF16, 2, 64, 64, 10, 16, 2 * 16 * 64, 16 * 64, 64, 2 * 16 * 64, 16 * 64, 64)
+    for k, v in kw.items():
+        setattr(g, k, v)
+    return g
+
+
+def batch(**kw):
+    b = mm.Batch(P, P, P, 4, 4, 3, 5, mm.MM_INT32)
+    for k, v in kw.items():
+        setattr(b, k, v)
+    return b
+
+
+def err(rc):
+    assert rc == mm.MM_ERR_ARG
+    return mm.last_error()
+
+
+def append(g=None, b=None, q=P, q_ts=512, q_hs=64, k=P, v=P, nh=14, inv=P, pairs=32, off=0, q_out=P, k_out=None):
+    g, b = g or pages(), b or batch()
+    return mm.load().mm_paged_append(q, q_ts, q_hs, k, 128, 64, v, 128, 64, nh, g, b, inv, pairs, off, 0, q_out, 896, 64,
+                                     k_out, 128, 64, None)
+
+
+def attn(g=None, b=None, q=P, q_ts=896, nh=14, out=P, o_hs=64, ws=P, ws_bytes=1 << 40):
+    return mm.load().mm_paged_attn(q, q_ts, 64, nh, g or pages(), b or batch(), 0.125, out, 896, o_hs, ws, ws_bytes, None)
+
+
+def prompt(q=P, k=P, v=P, dtype=mm.MM_BF16, nh=14, nkv=2, dqk=64, dv=64, cu=P, idx=mm.MM_INT32, seqs=3, tokens=5, out=P,
+           k_ts=128):
+    return mm.load().mm_prompt_attn(q, 896, 64, k, k_ts, 64, v, 128, 64, dtype, nh, nkv, dqk, dv, cu, idx, seqs, tokens,
+                                    0.125, out, 896, 64, P, 1 << 40, None)
+
+
+@pytest.mark.parametrize("call", [append, attn])
+@pytest.mark.parametrize("what,g,b", [
+    ("bf16 or fp16", dict(dtype=mm.MM_FP32), {}), ("multiple of nkv", dict(nkv=4), {}), ("multiple of nkv", dict(nkv=0), {}),
+    ("dqk=60", dict(dqk=60), {}), ("dqk=264", dict(dqk=264), {}), ("dv=0", dict(dv=0), {}), ("dv=260", dict(dv=260), {}),
+    ("page or table", dict(page=0), {}), ("page or table", dict(n_pages=-1), {}), ("page or table", {}, dict(max_pages=-1)),
+    ("below 2^31", dict(page=1 << 20), dict(max_pages=1 << 11)), ("tokens -1", {}, dict(tokens=-1)),
+    ("tokens", {}, dict(tokens=1 << 23)), ("streams", {}, dict(seqs=-1)), ("streams", {}, dict(seqs=1 << 21)),
+    ("int32 or int64", {}, dict(idx_dtype=mm.MM_FP32)), ("null batch", {}, dict(cu=None)),
+    ("null batch", {}, dict(kv_lens=None)), ("null batch", {}, dict(table=None)), ("null pool", dict(v=None), {}),
+    ("16-byte aligned", dict(k=P + 8), {}), ("multiples of 8", dict(k_row_stride=68), {}),
+    ("multiples of 8", dict(v_page_stride=-8), {})])
+def test_the_pool_and_the_batch_are_checked(call, what, g, b):
+    assert what in err(call(g=pages(**g), b=batch(**b)))
+
+
+def test_append_refuses():
+    assert "pairs" in err(append(pairs=36)) and "pairs" in err(append(pairs=40)) and "pairs" in err(append(off=8))
+    assert "pairs" in err(append(pairs=16, off=4)) and "pairs" in err(append(pairs=-8))
+    assert "null q" in err(append(q=None)) and "null k" in err(append(k=None)) and "null v" in err(append(v=None))
+    assert "null q_out" in err(append(q_out=None))
+    assert "q must be 16-byte" in err(append(q=P + 2)) and "k_out must be 16-byte" in err(append(k_out=P + 8))
+    assert "strides of q" in err(append(q_ts=900)) and "strides of q" in err(append(q_hs=-64))
+    assert "null descriptor" in err(mm.load().mm_paged_append(P, 896, 64, P, 128, 64, P, 128, 64, 14, None, None, P, 32, 0, 0,
+                                                              P, 896, 64, None, 0, 0, None))
+
+
+def test_attn_refuses():
+    assert "null q" in err(attn(q=None)) and "null out" in err(attn(out=None))
+    assert "strides of q" in err(attn(q_ts=892)) and "out must be 8-byte" in err(attn(out=P + 4))
+    assert "strides of out" in err(attn(o_hs=66))
+    need = mm.load().mm_paged_attn_workspace(5, 3, 64, 14, 2, 64, 64)
+    assert need >= 0
+    if need:
+        assert "workspace" in err(attn(ws_bytes=need - 1)) and "workspace" in err(attn(ws=None))
+        assert "workspace" in err(attn(ws=P + 4))
+
+
+def test_prompt_refuses():
+    assert "bf16 or fp16" in err(prompt(dtype=mm.MM_INT8)) and "multiple of nkv" in err(prompt(nh=15))
+    assert "dqk=68" in err(prompt(dqk=68)) and "dv=-8" in err(prompt(dv=-8)) and "null cu" in err(prompt(cu=None))
+    assert "int32 or int64" in err(prompt(idx=mm.MM_BF16)) and "tokens" in err(prompt(tokens=-3))
+    assert "streams" in err(prompt(seqs=-1)) and "null k" in err(prompt(k=None)) and "strides of k" in err(prompt(k_ts=129))
+    assert "out must be 8-byte" in err(prompt(out=P + 2))
+
+
+def test_nothing_to_do_is_done_without_a_gpu():
+    for b in (batch(tokens=0), batch(seqs=0)):
+        assert append(b=b) == 0 and attn(b=b) == 0
+    assert prompt(tokens=0) == 0 and prompt(seqs=0) == 0
+
+
+def test_workspace_sizes_are_refused_or_bounded():
+    lib = mm.load()
+    assert lib.mm_paged_attn_workspace(-1, 1, 64, 14, 2, 64, 64) == -1
+    assert lib.mm_paged_attn_workspace(1, 1, 1 << 31, 14, 2, 64, 64) == -1
+    assert lib.mm_paged_attn_workspace(1, 1, 64, 14, 4, 64, 64) == -1
+    assert lib.mm_prompt_attn_workspace(1, -1, 14, 2, 64, 64) == -1 and lib.mm_prompt_attn_workspace(1, 1, 14, 2, 64, 63) == -1
+    with pytest.raises(ValueError, match="dv=12"):
+        PK.prompt_attn_workspace(8, 2, 4, 2, 64, 12, device="cpu")
+    assert PK.paged_attn_workspace(1, 1, 64, 14, 2, 64, 64, device="cpu").numel() >= 16
+
+
+# ------------------------------------------------------------------------------------------------ refusals, wrappers
+
+def test_wrappers_take_gpu_tensors_only():
+    t, i = torch.zeros(1, 2, 64, dtype=BF), torch.zeros(2, dtype=torch.int32)
+    pool = torch.zeros(1, 2, 16, 64, dtype=BF)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    for call in (lambda: PK.paged_append(t, t, t, pool, pool, table, i, i[:1]),
+                 lambda: PK.paged_attn(t, pool, pool, table, i, i[:1]), lambda: PK.prompt_attn(t, t, t, i)):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+
+
+@pytest.fixture
+def any_device(monkeypatch):
+    """The wrappers' own checks on CPU tensors: none of the refused calls reaches the library."""
+    monkeypatch.setattr(mm, "require_gpu", lambda *t: None)
+
+
+def _args(N=3, B=2, nh=4, nkv=2, d=16, dv=8, dt=BF, idx=torch.int32):
+    return dict(q=torch.zeros(N, nh, d, dtype=dt), k=torch.zeros(N, nkv, d, dtype=dt), v=torch.zeros(N, nkv, dv, dtype=dt),
+                k_pages=torch.zeros(5, nkv, 4, d, dtype=dt), v_pages=torch.zeros(5, nkv, 4, dv, dtype=dt),
+                page_table=torch.zeros(B, 3, dtype=idx), cu_seqlens=torch.zeros(B + 1, dtype=idx),
+                kv_lens=torch.zeros(B, dtype=idx))
+
+
+@pytest.mark.parametrize("what,change", [
+    ("q must be", dict(q=torch.zeros(3, 4, 24, dtype=BF))), ("q must be", dict(q=torch.zeros(3, 64, dtype=BF))),
+    ("q must be", dict(q=torch.zeros(3, 4, 16))), ("contiguous last dim", dict(q=torch.zeros(3, 16, 4, dtype=BF).mT)),
+    ("k must be", dict(k=torch.zeros(3, 3, 16, dtype=BF))), ("v must be", dict(v=torch.zeros(3, 2, 16, dtype=BF))),
+    ("same tokens", dict(k=torch.zeros(4, 2, 16, dtype=BF))),
+    ("k_pages and v_pages must be", dict(k_pages=torch.zeros(5, 2, 8, 16, dtype=BF))),
+    ("both be bf16 or fp16", dict(k_pages=torch.zeros(5, 2, 4, 16))),
+    ("kv_lens must be", dict(kv_lens=torch.zeros(3, dtype=torch.int32))),
+    ("one dtype", dict(kv_lens=torch.zeros(2, dtype=torch.int64))), ("cu_seqlens", dict(cu_seqlens=torch.zeros(3))),
+    ("cu_seqlens", dict(cu_seqlens=torch.zeros(0, dtype=torch.int32))),
+    ("page_table", dict(page_table=torch.zeros(3, 3, dtype=torch.int32))),
+    ("page_table", dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t())),
+    ("inv_freq", dict(inv_freq=torch.zeros(8, dtype=BF))), ("q_out", dict(q_out=torch.zeros(3, 4, 8, dtype=BF))),
+    ("q_out must hold 3", dict(q_out=torch.zeros(2, 4, 16, dtype=BF))),
+    ("k_out must hold 3", dict(k_out=torch.zeros(2, 2, 16, dtype=BF)))])
+def test_append_wrapper_refuses(any_device, what, change):
+    with pytest.raises(ValueError, match=what):
+        PK.paged_append(**{**_args(), **change})
+
+
+@pytest.mark.parametrize("what,change", [
+    ("q must be", dict(q=torch.zeros(3, 4, 24, dtype=BF))), ("q must be", dict(q=torch.zeros(3, 4, 16, dtype=torch.float16))),
+    ("k_pages and v_pages must be", dict(v_pages=torch.zeros(4, 2, 4, 8, dtype=BF))),
+    ("out must hold 3", dict(out=torch.zeros(2, 4, 8, dtype=BF))), ("out must be", dict(out=torch.zeros(3, 4, 16, dtype=BF))),
+    ("one dtype", dict(page_table=torch.zeros(2, 3, dtype=torch.int64)))])
+def test_attn_wrapper_refuses(any_device, what, change):
+    a = {k: v for k, v in _args().items() if k not in "kv"}
+    with pytest.raises(ValueError, match=what):
+        PK.paged_attn(**{**a, **change})
+
+
+@pytest.mark.parametrize("what,change", [
+    ("bf16 or fp16", dict(q=torch.zeros(3, 4, 16))), ("k must be", dict(k=torch.zeros(3, 2, 8, dtype=BF))),
+    ("v must be", dict(v=torch.zeros(3, 1, 8, dtype=BF))), ("same tokens", dict(v=torch.zeros(2, 2, 8, dtype=BF))),
+    ("cu_seqlens", dict(cu_seqlens=torch.zeros(2, 2, dtype=torch.int32))),
+    ("out must be", dict(out=torch.zeros(3, 4, 8)))])
+def test_prompt_wrapper_refuses(any_device, what, change):
+    a = {k: v for k, v in _args().items() if k in ("q", "k", "v", "cu_seqlens")}
+    with pytest.raises(ValueError, match=what):
+        PK.prompt_attn(**{**a, **change})
+
+
+# ------------------------------------------------------------------------------------------------ arithmetic
+
+def test_division_by_a_page_is_exact():
+    """The kernels' n / d: umulhi(n, floor(2^(31 + l) / d) + 1) >> (l - 1), l = ceil(log2 d), for n < 2^31."""
+    for d in [2, 3, 5, 7, 14, 16, 24, 25, 100, 255, 256, 641, 1000, 4096, 65537, 1 << 20, (1 << 30) + 1, (1 << 31) - 1]:
+        length = (d - 1).bit_length()
+        m = (1 << (31 + length)) // d + 1
+        assert m < 1 << 32
+        top = (1 << 31) - 1
+        for n in {0, 1, d - 1, d, d + 1, top, top - 1, top // d * d, top // d * d - 1, 12345678, top // 2}:
+            if 0 <= n <= top:
+                assert ((n * m) >> 32) >> (length - 1) == n // d, (n, d)
+
+
+def test_oracle_matches_torch_attention():
+    torch.manual_seed(0)
+    q, k, v = (torch.randn(7, n, 16, dtype=torch.float64) for n in (4, 2, 2))
+    cu = torch.tensor([0, 3, 3, 7])
+    out, _, _ = O.prompt_attn(q, k, v, cu, 0.3)
+    for a, b in ((0, 3), (3, 7)):
+        qs, ks, vs = q[a:b].transpose(0, 1), *(t[a:b].repeat_interleave(2, 1).transpose(0, 1) for t in (k, v))
+        want = torch.nn.functional.scaled_dot_product_attention(qs, ks, vs, is_causal=True, scale=0.3)
+        torch.testing.assert_close(out[a:b], want.transpose(0, 1))
+    # the same rows in pages of 2, as a chunk of the last two tokens behind what came before, and a page that is missing
+    pool_k, pool_v = (torch.randn(6, 2, 2, 16, dtype=torch.float64) for _ in range(2))
+    table = torch.tensor([[4, 1], [9, 9], [0, 3]])
+    for b, (a, e) in enumerate(((0, 3), (3, 3), (3, 7))):
+        for p in range(e - a):
+            pool_k[table[b, p // 2], :, p % 2], pool_v[table[b, p // 2], :, p % 2] = k[a + p], v[a + p]
+    part = torch.cat([q[1:3], q[5:7]])
+    got, _, _ = O.paged_attn(part, pool_k, pool_v, table, torch.tensor([0, 2, 2, 4]), torch.tensor([3, 0, 4]), 0.3)
+    torch.testing.assert_close(got, torch.cat([out[1:3], out[5:7]]))
+    table[0, 0] = -1
+    got, _, _ = O.paged_attn(part, pool_k, pool_v, table, torch.tensor([0, 2, 2, 4]), torch.tensor([3, 0, 4]), 0.3)
+    assert (got[0] == 0).all()  # its only positions lie in the missing page
+    torch.testing.assert_close(got[1], v[2].repeat_interleave(2, 0))
