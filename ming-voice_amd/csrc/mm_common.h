@@ -366,4 +366,75 @@ __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((n & 15) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8));
 }
 
+// Orders a wave's LDS stores before its later loads (and loads before later stores) without a workgroup barrier:
+// a wave's LDS instructions execute in program order, so only the compiler's reordering has to be fenced.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The LDS address of a pointer into shared memory, as LDS instructions take it.
+__device__ __forceinline__ uint32_t lds_place(const char* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// Every LDS read of the wave has returned (and none moves past): its source may be overwritten.
+__device__ __forceinline__ void wait_lgkm0() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (0x7 << 4) | (0 << 8));
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// v, or zero when !ok (a select per dword, no branch)
+__device__ __forceinline__ uint4 and_mask16(const uint4& v, bool ok) {
+  const uint32_t m = ok ? ~0u : 0u;
+  return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
+}
+
+// ---- pieces of the attention kernels
+
+// 8 bytes per lane from LDS, transposed within groups of 16 lanes: with lane s of a group reading row s / 4, columns
+// 4 (s % 4) .. + 3 of a 4 x 16 block of bf16, lane i receives column i of the 4 rows (ds_read_b64_tr_b16; the lane layout
+// checked on the device). Four fragments at once, each from place p[i] and `HI` bytes on, waited for in the same block:
+// the builtin makes the compiler wait for every load in flight into LDS, the next tile's among them.
+template <int HI>
+__device__ __forceinline__ void lds_tr4x2(const uint32_t (&p)[4], uint64_t (&lo)[4], uint64_t (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+      : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(HI)
+      : "memory");
+}
+
+__device__ __forceinline__ bf16x8_t lds_frag(const char* p) {
+  return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(p));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Max over the 4 lanes that share lane % 16.
+__device__ __forceinline__ float quarter_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), true, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), true, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The chunk of a tile's row held at LDS place c of the row (an involution). Keys: the 16 rows that a fragment reads at
+// one chunk fall on the 16 distinct 16-byte columns of the banks; values: the 16 rows of a transposing read, 32 bytes
+// each, fall on the 8 columns twice.
+template <int KC>
+__device__ __forceinline__ int k_chunk_at(int row, int c) {
+  return KC % 16 == 0 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
+}
+template <int VC>
+__device__ __forceinline__ int v_chunk_at(int row, int c) {
+  return VC % 16 == 0 ? c ^ (2 * (row & 7)) : c ^ (2 * ((row >> 1) & 3));
+}
+
 }  // namespace mmd

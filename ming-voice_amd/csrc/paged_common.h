@@ -1,0 +1,311 @@
+// What the kernels of the paged cache share: the batch on the device, page arithmetic, the arguments of an attention and
+// the division of its work over workgroups.
+#pragma once
+
+#include "mingpaged.h"
+#include "mm_common.h"
+
+namespace mmp {
+
+using namespace mmd;
+
+// n / d for n < 2^31 by a multiplication: m = floor(2^(31 + l) / d) + 1 with l = ceil(log2 d) exceeds 2^(31 + l) / d by at
+// most 1 <= 2^l / d, so the product is off by less than 1 / d for every such n.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+};
+
+inline FastDiv fast_div(int64_t d) {
+  FastDiv f{static_cast<uint32_t>(d), 0, 0};
+  if (d > 1) {
+    int l = 0;
+    while ((1LL << l) < d) ++l;
+    f.m = static_cast<uint32_t>((1ULL << (31 + l)) / static_cast<uint64_t>(d) + 1);
+    f.s = l - 1;
+  }
+  return f;
+}
+
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return f.d == 1 ? n : __umulhi(n, f.m) >> f.s;
+}
+
+// The batch as the kernels see it: device arrays of one index type, every value clamped before use, so that no content of
+// them leads outside a buffer.
+struct Batch {
+  const void* cu;
+  const void* lens;
+  const void* table;
+  int64_t table_stride;
+  int i64;          // the arrays hold 64-bit numbers
+  int seqs, tokens;
+  int max_keys;     // max_pages * page
+};
+
+__device__ __forceinline__ int64_t idx_at(const void* p, int i64, int64_t i) {
+  return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// A stream's first token, the number of its tokens and the rows of its cache that count (-1: outside the table).
+struct Stream {
+  int first, n, kv;
+};
+
+__device__ __forceinline__ Stream stream_at(const Batch& a, int b) {
+  const int64_t c0 = idx_at(a.cu, a.i64, b), c1 = idx_at(a.cu, a.i64, b + 1);
+  Stream s;
+  s.first = static_cast<int>(min(max(c0, static_cast<int64_t>(0)), static_cast<int64_t>(a.tokens)));
+  s.n = static_cast<int>(min(max(c1, static_cast<int64_t>(s.first)), static_cast<int64_t>(a.tokens))) - s.first;
+  if (a.lens) {
+    const int64_t kv = idx_at(a.lens, a.i64, b);
+    s.kv = kv < 0 || kv > a.max_keys ? -1 : static_cast<int>(kv);
+  } else {
+    s.kv = s.n;  // a prompt's own rows
+  }
+  return s;
+}
+
+// The stream that token t belongs to (seqs: none), found by the whole wave: the number of streams that end at or before t.
+__device__ __forceinline__ int stream_of_token(const Batch& a, int t) {
+  int b = 0;
+  for (int base = 0; base < a.seqs; base += kWave) {
+    const int i = base + lane_id();
+    const bool before = i < a.seqs && idx_at(a.cu, a.i64, min(i, a.seqs - 1) + 1) <= t;
+    const int n = __popcll(__ballot(before));
+    b += n;
+    if (n < kWave) break;
+  }
+  return min(b, a.seqs);
+}
+
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::kBf16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      x[2 * i] = f16_to_f32(static_cast<uint16_t>(w[i]));
+      x[2 * i + 1] = f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (T::kBf16) return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
+  else return static_cast<uint32_t>(f32_to_f16(lo)) | (static_cast<uint32_t>(f32_to_f16(hi)) << 16);
+}
+
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+}
+
+__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void st16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// Rows [tokens, heads, d] of a packed tensor, or one page's: element strides.
+struct Rows {
+  uint16_t* p;
+  int64_t ts, hs;
+  __device__ __forceinline__ uint16_t* at(int64_t t, int h) const { return p + t * ts + h * hs; }
+};
+
+struct Pool {
+  uint16_t* p;
+  int64_t ps, hs, rs;
+  __device__ __forceinline__ uint16_t* at(int64_t page, int h, int row) const { return p + page * ps + h * hs + row * rs; }
+};
+
+// ------------------------------------------------------------------------------------------ attention
+
+struct AttnArgs {
+  Rows q, out;
+  Rows k, v;    // a prompt's packed rows
+  Pool kp, vp;  // the cache
+  Batch batch;
+  FastDiv page, group;  // group: query heads of a key / value head
+  int n_pages;
+  int nh, nkv, dqk, dv;
+  float scale;       // its size; negative scales turn the queries' sign
+  int negative;
+  int target;        // pieces of the keys aimed at, 0: every row block takes all its keys at once
+  float* ws;         // the pieces' states
+};
+
+// How the work is divided. A row is one token's query at one of the G heads that share a key / value head (row r of a
+// stream: token r / G, head r % G), so that a block of BR rows reads each key once for all of them. A stream of n tokens
+// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys are cut into pieces of `cut` granules of GR keys:
+// cut is the smallest for which the sum over all blocks of (granules / cut) stays within target, so the pieces are of one
+// length whatever the streams' lengths are, and a long stream among short ones is shared by many workgroups. Only blocks
+// of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there are at most 2 target of them, a bound that needs
+// no length on the host. Workgroups are at most target + blocks.
+struct Work {
+  int b, blk;      // stream (-1: none) and row block
+  int piece;       // of the block's keys
+  int cut;         // granules in a piece
+  int slot;        // state of the block's first piece
+  Stream s;
+};
+
+template <int BR>
+__device__ __forceinline__ int blocks_of(const Stream& s, int group) {
+  return (s.n * group + BR - 1) / BR;
+}
+
+// Keys that the rows r0 .. r0 + BR - 1 of a stream see together (its rows end at n G), and the pieces they make.
+template <int BR>
+__device__ __forceinline__ int keys_of(const Stream& s, int blk, const FastDiv& group) {
+  const int last = min(blk * BR + BR, s.n * static_cast<int>(group.d)) - 1;
+  return s.kv < 0 ? 0 : max(0, s.kv - s.n + static_cast<int>(div_by(last, group)) + 1);
+}
+
+template <int GR>
+__device__ __forceinline__ int pieces_of(int keys, int cut) {
+  const int g = (keys + GR - 1) / GR;
+  return cut == 0 ? 1 : max(1, (g + cut - 1) / cut);
+}
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int o = __shfl_up(v, d, kWave);
+    v += lane_id() >= d ? o : 0;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int64_t wave_total(int64_t v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
+  return v;
+}
+
+// The work of workgroup w (BY_BLOCK: of row block w, piece 0), found by every wave from the batch itself: streams 64 at a
+// time, one to a lane. Within a stream the last row block, whose rows see the most keys, comes first.
+template <int BR, int GR, bool BY_BLOCK>
+__device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
+  const int G = static_cast<int>(a.group.d), lane = lane_id(), B = a.batch.seqs;
+  Work k{-1, 0, 0, 0, 0, Stream{0, 0, 0}};
+  Stream mine{0, 0, 0};
+  auto load = [&](int base) {
+    mine = Stream{0, 0, 0};
+    if (base + lane < B) mine = stream_at(a.batch, base + lane);
+  };
+  load(0);
+  if (a.target > 0) {
+    int64_t total = 0;
+    for (int base = 0; base < B; base += kWave) {
+      if (base) load(base);
+      total += static_cast<int64_t>(blocks_of<BR>(mine, G)) * ((max(mine.kv, 0) + GR - 1) / GR);
+    }
+    total = wave_total(total);
+    k.cut = static_cast<int>(max((total + a.target - 1) / a.target, static_cast<int64_t>(1)));
+    if (B > kWave) load(0);
+  }
+  int slots = 0;
+  for (int base = 0; base < B; base += kWave) {
+    if (base) load(base);
+    const int blocks = blocks_of<BR>(mine, G), pieces = pieces_of<GR>(max(mine.kv, 0), k.cut);
+    const int units = BY_BLOCK ? blocks : blocks * pieces, held = pieces > 1 ? blocks * pieces : 0;
+    const int ends = wave_scan(units), last = __builtin_amdgcn_readlane(ends, kWave - 1);
+    if (w < last) {
+      const int src = __ffsll(static_cast<long long>(__ballot(ends > w))) - 1;
+      const int held_before = wave_scan(held) - held;
+      const int u = w - (__builtin_amdgcn_readlane(ends, src) - __builtin_amdgcn_readlane(units, src));
+      const int p = __builtin_amdgcn_readlane(pieces, src), nb = __builtin_amdgcn_readlane(blocks, src);
+      const int at = BY_BLOCK ? u : u / p;
+      k.b = base + src;
+      k.s = Stream{__builtin_amdgcn_readlane(mine.first, src), __builtin_amdgcn_readlane(mine.n, src),
+                   __builtin_amdgcn_readlane(mine.kv, src)};
+      k.blk = nb - 1 - at;
+      k.piece = BY_BLOCK ? 0 : u - at * p;
+      k.slot = slots + __builtin_amdgcn_readlane(held_before, src) + at * p;
+      // always so for a cu that does not fall; one that does must not lead out of the buffers either
+      if (u < 0 || at >= nb || (p > 1 && (k.slot < 0 || k.slot + p > 2 * a.target))) k.b = -1;
+      return k;
+    }
+    w -= last;
+    slots += __builtin_amdgcn_readlane(wave_scan(held), kWave - 1);
+  }
+  return k;
+}
+
+// find_work's answer as the scalars that it is: what follows branches on them, and a matrix instruction, which pays no heed
+// to the lanes' mask, must stand behind scalar branches only.
+__device__ __forceinline__ Work scalars(const Work& w) {
+  auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return Work{u(w.b), u(w.blk), u(w.piece), u(w.cut), u(w.slot), Stream{u(w.s.first), u(w.s.n), u(w.s.kv)}};
+}
+
+// A state: BR rows of dv sums, then the rows' maxima (in units of log2 of the weight), then their sums.
+template <int BR>
+__device__ __forceinline__ float* state_at(const AttnArgs& a, int slot, int kvh) {
+  return a.ws + (static_cast<int64_t>(slot) * a.nkv + kvh) * BR * (a.dv + 2);
+}
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+template <class T>
+struct Mfma;
+template <>
+struct Mfma<BF16> {
+  typedef bf16x8_t V;
+  static __device__ __forceinline__ floatx4 m16(const uint4& a, const uint4& b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ floatx16 m32(const uint4& a, const uint4& b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t kExp = 0x7f807f80u;  // the exponents of a pair
+};
+template <>
+struct Mfma<FP16> {
+  typedef _Float16 V __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ floatx4 m16(const uint4& a, const uint4& b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ floatx16 m32(const uint4& a, const uint4& b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t kExp = 0x7c007c00u;
+};
+
+// Whether a pair of values holds an infinity or a NaN.
+template <class T>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  constexpr uint32_t lo = Mfma<T>::kExp & 0xffffu, hi = Mfma<T>::kExp & 0xffff0000u;
+  return (w & lo) == lo || (w & hi) == hi;
+}
+
+// The page number read for a key, as it came (both halves of a 64-bit entry; the same word twice of a 32-bit one), so
+// that nothing waits for it before it is used.
+struct PageId {
+  uint32_t lo, hi;
+};
+
+__device__ __forceinline__ PageId page_id(const AttnArgs& a, int b, int key) {
+  const int64_t i = b * a.batch.table_stride + div_by(key, a.page);
+  const uint32_t* p = static_cast<const uint32_t*>(a.batch.table) + (a.batch.i64 ? 2 * i : i);
+  return PageId{p[0], p[a.batch.i64 ? 1 : 0]};
+}
+
+__device__ __forceinline__ bool page_ok(const AttnArgs& a, PageId id) {
+  return static_cast<int>(id.lo) >= 0 && static_cast<int>(id.lo) < a.n_pages && (!a.batch.i64 || id.hi == 0);
+}
+
+// What a row that does not exist reads.
+static __device__ const uint4 kZeroRow[32] = {};
+
+// The attention of blocks of few rows (16), whose waves share out the keys.
+struct FewPlan {
+  int64_t blocks, target, workspace;
+};
+FewPlan plan_few(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+int launch_few(AttnArgs& a, const FewPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
+
+}  // namespace mmp

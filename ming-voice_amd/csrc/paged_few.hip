@@ -1,0 +1,426 @@
+// Attention of few rows over many keys (decode steps, short pieces): 16 rows to a workgroup, the keys shared out among its
+// waves, and among workgroups where the keys are many (paged_common.h: find_work).
+#include "paged_common.h"
+
+namespace mmp {
+
+namespace {
+
+constexpr int kKeys = 32;  // keys per tile
+
+// The shape of few_kernel: QF 16-row fragments, NW waves, head dims up to 32 NKQ (q, k) and 16 NT (v).
+template <int QF, int NW, int NKQ, int NT>
+struct Few {
+  static constexpr int BR = 16 * QF;
+  static constexpr int GR = NW * kKeys;                  // a granule: a tile for every wave
+  static constexpr int DVM = 16 * NT;
+  static constexpr int KC = 4 * NKQ, VC = 2 * NT;        // 16-byte chunks of a key, value row in LDS
+  static constexpr int KI = kKeys * KC / kWave, VI = kKeys * VC / kWave;  // loads per key, value tile
+  static constexpr int K_BYTES = kKeys * KC * 16, V_BYTES = kKeys * VC * 16;
+  static constexpr int OROW = DVM + 4;
+  static constexpr int ML = BR * OROW;                   // the wave's maxima and sums, after its outputs
+  static constexpr int O_BYTES = (ML + 2 * BR) * 4;
+  static constexpr int WAVE_BYTES = K_BYTES + V_BYTES > O_BYTES ? K_BYTES + V_BYTES : O_BYTES;
+  static constexpr size_t LDS = static_cast<size_t>(NW) * WAVE_BYTES;
+  static_assert(LDS <= 160 * 1024 && KI % 2 == 0 && NT % 4 == 0, "tile shape");
+};
+
+// Softmax attention of up to 16 QF rows over a piece of their keys, one pass with a running maximum and sum. Grid (work,
+// key / value heads) x NW waves. Wave w takes tiles w, w + NW, ... of 32 keys of the piece; the waves' states meet in LDS.
+// Per tile, on the 16x16x32 MFMA (bf16 or fp16, fp32 sums):
+//   S^T [32 keys, 16 rows] = K Q^T: the key rows as A fragments from LDS, the rows' queries held as B fragments;
+//   the softmax update per row is lane-local (a lane of S^T holds 8 keys of row lane % 16), the maximum over 4 lanes;
+//   O^T [dv, 16 rows] += V^T P^T: P^T straight from the S^T registers (weights rounded to the cache's type: the matrix
+//     units' operand, 2^-9 of a weight), V^T by transposing LDS reads.
+// Bound by the cache rows' way from memory: they come by loads straight into the wave's own LDS, the next tile's keys
+// requested as soon as this one's are in registers, its values as soon as this one's are; the page numbers of the tile
+// after that are read one tile ahead, lane l for key l % 32, and handed to the loading lanes by ds_bpermute. Keys that no
+// row sees (past the piece, in a missing page) read a row of zeros. A value that some rows must not see could still be an
+// infinity or NaN (0 * inf): such tiles take their values key by key (spill_safe below).
+template <class T, int QF, int NW, int NKQ, int NT, bool PAGED>
+__global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
+  using P = Few<QF, NW, NKQ, NT>;
+  constexpr int BR = P::BR;
+  extern __shared__ __align__(16) char s_few[];
+  const int tid = threadIdx.x, lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lr = lane & 15, lq = lane >> 4, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
+  const Work w = scalars(find_work<BR, P::GR, false>(a, blockIdx.x));
+  if (w.b < 0) return;
+  const int r0 = w.blk * BR, rows = min(BR, w.s.n * G - r0), n4 = a.dv / 4;
+  auto out_at = [&](int r) {  // row r0 + r of the stream
+    const int i = static_cast<int>(div_by(r0 + r, a.group));
+    return a.out.at(w.s.first + i, kvh * G + (r0 + r - i * G));
+  };
+  if (w.s.kv < 0) {
+    for (int i = tid; i < rows * a.dv; i += NW * kWave) T::st(out_at(i / a.dv), i % a.dv, NAN);
+    return;
+  }
+  const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<P::GR>(keys, w.cut);
+  if (w.piece >= pieces) return;
+  const int k_begin = w.piece * w.cut * P::GR;  // one piece: 0
+  const int k_end = w.cut == 0 ? keys : min(keys, k_begin + w.cut * P::GR);
+  const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;
+  char* kt = s_few + wave * P::WAVE_BYTES;
+  char* vt = kt + P::K_BYTES;
+  // load i of a key tile fills LDS chunks 64 i + lane: row krow[i % KH] (+ 16 for the second half), dims kdim[i % KH] ..;
+  // of a value tile row vrow + VPI i, dims vdim[i % VP] ..
+  constexpr int KH = P::KI / 2, VPI = kWave / P::VC, VP = P::VC == 32 ? 4 : 2;
+  int krow[KH], kdim[KH], vdim[VP];
+#pragma unroll
+  for (int i = 0; i < KH; ++i) {
+    krow[i] = (kWave * i + lane) / P::KC;
+    kdim[i] = 8 * k_chunk_at<P::KC>(krow[i], (kWave * i + lane) % P::KC);
+  }
+  const int vrow = lane / P::VC;
+#pragma unroll
+  for (int i = 0; i < VP; ++i) vdim[i] = 8 * v_chunk_at<P::VC>(vrow + VPI * i, lane % P::VC);
+
+  const char* zeros = reinterpret_cast<const char*>(kZeroRow);
+  // lane l's key of a tile, clamped into the piece
+  auto key_of = [&](int it) { return min(k_begin + it * kKeys + (lane & (kKeys - 1)), k_end - 1); };
+  // the rows of a tile's keys: lane l's key and value row, and which of the 32 exist
+  const char *kr, *vr;
+  uint32_t there = 0;
+  auto find_rows = [&](int it, PageId id) {
+    const int key = k_begin + it * kKeys + (lane & (kKeys - 1));
+    bool ok = key < k_end;
+    const int kc = min(key, k_end - 1);
+    if constexpr (PAGED) {
+      ok = ok && page_ok(a, id);
+      const int row = kc - static_cast<int>(div_by(kc, a.page)) * static_cast<int>(a.page.d);
+      kr = reinterpret_cast<const char*>(a.kp.at(static_cast<int>(id.lo), kvh, row));
+      vr = reinterpret_cast<const char*>(a.vp.at(static_cast<int>(id.lo), kvh, row));
+    } else {
+      kr = reinterpret_cast<const char*>(a.k.at(w.s.first + kc, kvh));
+      vr = reinterpret_cast<const char*>(a.v.at(w.s.first + kc, kvh));
+    }
+    if (!ok) kr = vr = zeros;
+    there = static_cast<uint32_t>(__ballot(ok));
+  };
+  auto row_of = [&](const char* p, int r) {  // row r's address, from the lane that found it
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * r, static_cast<int>(v)));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * r, static_cast<int>(v >> 32)));
+    return reinterpret_cast<const char*>((static_cast<uint64_t>(hi) << 32) | lo);
+  };
+  auto load_k = [&] {
+#pragma unroll
+    for (int i = 0; i < P::KI; ++i) {
+      const char* p = row_of(kr, krow[i % KH] + (i / KH) * 16) + 2 * kdim[i % KH];
+      load_lds16(kdim[i % KH] < a.dqk ? p : zeros, kt + i * 1024);
+    }
+  };
+  auto load_v = [&] {
+#pragma unroll
+    for (int i = 0; i < P::VI; ++i) {
+      const char* p = row_of(vr, vrow + VPI * i) + 2 * vdim[i % VP];
+      load_lds16(vdim[i % VP] < a.dv ? p : zeros, vt + i * 1024);
+    }
+  };
+  // LDS places of this lane's fragment pieces: key row 16 f + lr, chunk 4 kk + lq; value rows 4 lq + lr / 4 (+ 16), dims
+  // 16 nt + 4 (lr % 4) .. + 3
+  const char* kfrag = kt + lr * P::KC * 16;
+  const int vfr = 4 * lq + lr / 4;
+  const int vplace = vfr * P::VC * 16 + v_chunk_at<P::VC>(vfr, (lr % 4) / 2) * 16 + (lr & 1) * 8;
+
+  uint4 qf[QF][NKQ];
+  int lim[QF];  // keys that this lane's row sees
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    const int r = r0 + min(16 * f + lr, rows - 1), i = static_cast<int>(div_by(r, a.group));
+    const uint16_t* qrow = a.q.at(w.s.first + i, kvh * G + (r - i * G));
+    lim[f] = w.s.kv - w.s.n + i + 1;
+#pragma unroll
+    for (int kk = 0; kk < NKQ; ++kk) {
+      const int d = 32 * kk + 8 * lq;
+      const bool ok = d < a.dqk;
+      uint4 x = and_mask16(ld16(qrow + (ok ? d : 0)), ok);
+      const uint32_t sign = a.negative ? 0x80008000u : 0u;
+      qf[f][kk] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+    }
+  }
+  const int lim_all = w.s.kv - w.s.n + static_cast<int>(div_by(r0, a.group)) + 1;  // keys that every row sees
+  floatx4 o[QF][NT];
+  float m[QF], l[QF];
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    m[f] = -INFINITY;
+    l[f] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) o[f][nt] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float sc = a.scale * 1.4426950408889634f;  // scores in units of log2: exp2 gives the weights
+  if (wave < tiles) {
+    PageId next{0, 0};
+    if constexpr (PAGED) next = page_id(a, w.b, key_of(wave));
+    find_rows(wave, next);
+    if constexpr (PAGED) next = page_id(a, w.b, key_of(wave + NW));
+    wait_vmcnt<0>();  // the queries and pages: from here on only tiles and page numbers are in flight
+    load_k();
+    load_v();
+    for (int it = wave; it < tiles; it += NW) {
+      const int j0 = k_begin + it * kKeys;
+      const uint32_t mine = there;  // the tile's keys that exist
+      wait_vmcnt<P::VI>();  // the tile's keys (its values still in flight)
+      wave_lds_fence();
+      uint4 kx[2][NKQ];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kk = 0; kk < NKQ; ++kk)
+          kx[u][kk] = *reinterpret_cast<const uint4*>(kfrag + u * 16 * P::KC * 16 + k_chunk_at<P::KC>(lr, 4 * kk + lq) * 16);
+      wait_lgkm0();  // read before the next tile overwrites them
+      const bool more = it + NW < tiles;
+      if (more) {
+        find_rows(it + NW, next);
+        if constexpr (PAGED) next = page_id(a, w.b, key_of(it + 2 * NW));
+        load_k();
+      }
+      floatx4 s[QF][2];
+#pragma unroll
+      for (int f = 0; f < QF; ++f) s[f][0] = s[f][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < NKQ; ++kk)
+#pragma unroll
+        for (int f = 0; f < QF; ++f)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s[f][u] = Mfma<T>::m16(kx[u][kk], qf[f][kk], s[f][u]);
+      const bool mixed = j0 + kKeys > lim_all;  // some row does not see some key that exists
+      uint32_t sees[QF];
+      uint4 pf[QF];
+#pragma unroll
+      for (int f = 0; f < QF; ++f) {
+        const int n = lim[f] - j0;
+        sees[f] = n >= kKeys ? mine : n <= 0 ? 0u : mine & ((1u << n) - 1u);
+        const uint32_t lo4 = sees[f] >> (4 * lq), hi4 = sees[f] >> (16 + 4 * lq);
+        float sv[8];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // slot e < 4 is key 4 lq + e of the tile, slot e >= 4 key 16 + 4 lq + e - 4
+          const bool see = e < 4 ? (lo4 >> e) & 1u : (hi4 >> (e - 4)) & 1u;
+          sv[e] = see ? (e < 4 ? s[f][0][e] : s[f][1][e - 4]) * sc : -INFINITY;
+          tmax = fmaxf(tmax, sv[e]);
+        }
+        const float mn = fmaxf(m[f], quarter_max(tmax));
+        const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
+        const float alpha = exp2_fast(m[f] - mu);
+        m[f] = mn;
+        float ps = 0.f;
+        uint32_t pw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = exp2_fast(sv[2 * e] - mu), p1 = exp2_fast(sv[2 * e + 1] - mu);
+          ps += p0 + p1;
+          pw[e] = pack2<T>(p0, p1);
+        }
+        l[f] = fmaf(l[f], alpha, ps);
+        pf[f] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[f][nt] *= alpha;
+        }
+      }
+      if (more) wait_vmcnt<P::KI>();  // the tile's values (the next tile's keys still in flight)
+      else wait_vmcnt<0>();
+      wave_lds_fence();
+#pragma unroll
+      for (int n0 = 0; n0 < NT; n0 += 4) {
+        uint32_t place[4];
+        uint64_t lo[4], hi[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) place[b] = lds_place(vt) + (vplace ^ (32 * (n0 + b)));
+        lds_tr4x2<16 * P::VC * 16>(place, lo, hi);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint4 vf = make_uint4(static_cast<uint32_t>(lo[b]), static_cast<uint32_t>(lo[b] >> 32),
+                                      static_cast<uint32_t>(hi[b]), static_cast<uint32_t>(hi[b] >> 32));
+          // 0 * inf is NaN: where a row must not see a key whose value is not finite, the keys go one by one
+          if (mixed && __any(not_finite<T>(vf.x) || not_finite<T>(vf.y) || not_finite<T>(vf.z) || not_finite<T>(vf.w))) {
+#pragma unroll
+            for (int f = 0; f < QF; ++f) {
+              const uint32_t w0 = pf[f].x, w1 = pf[f].y, w2 = pf[f].z, w3 = pf[f].w;
+#pragma unroll 1
+              for (int key = 0; key < kKeys; ++key) {
+                const int e = key % 4 + 4 * (key / 16);
+                const uint32_t pw = e < 2 ? w0 : e < 4 ? w1 : e < 6 ? w2 : w3;
+                const uint32_t pk = static_cast<uint32_t>(
+                    __builtin_amdgcn_ds_bpermute(4 * (lr + 16 * (key % 16 / 4)), static_cast<int>(pw)));
+                const uint16_t pb = static_cast<uint16_t>(e & 1 ? pk >> 16 : pk);
+                const float p = T::kBf16 ? bf16_to_f32(pb) : f16_to_f32(pb);
+                const int d = 16 * (n0 + b) + 4 * lq;
+                const uint16_t* v = reinterpret_cast<const uint16_t*>(vt + key * P::VC * 16 +
+                                                                      v_chunk_at<P::VC>(key, d / 8) * 16) + d % 8;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float x = T::kBf16 ? bf16_to_f32(v[j]) : f16_to_f32(v[j]);
+                  o[f][n0 + b][j] = (sees[f] >> key) & 1u ? fmaf(p, x, o[f][n0 + b][j]) : o[f][n0 + b][j];
+                }
+              }
+            }
+            continue;
+          }
+#pragma unroll
+          for (int f = 0; f < QF; ++f) o[f][n0 + b] = Mfma<T>::m16(vf, pf[f], o[f][n0 + b]);
+        }
+      }
+      wait_lgkm0();  // read before the next tile overwrites them
+      if (more) load_v();
+    }
+  }
+  // the wave's state into its own LDS region, then the merge
+  float* so = reinterpret_cast<float*>(s_few + wave * P::WAVE_BYTES);
+  wave_lds_fence();
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    l[f] += __shfl_xor(l[f], 16, kWave);
+    l[f] += __shfl_xor(l[f], 32, kWave);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      *reinterpret_cast<floatx4*>(so + (16 * f + lr) * P::OROW + 16 * nt + 4 * lq) = o[f][nt];
+    if (lq == 0) {
+      so[P::ML + 16 * f + lr] = m[f];
+      so[P::ML + BR + 16 * f + lr] = l[f];
+    }
+  }
+  __syncthreads();
+  float* state = pieces > 1 ? state_at<BR>(a, w.slot + w.piece, kvh) : nullptr;
+  for (int i = tid; i < rows * n4; i += NW * kWave) {
+    const int r = i / n4, d = 4 * (i - r * n4);
+    auto of = [&](int x) { return reinterpret_cast<const float*>(s_few + x * P::WAVE_BYTES); };
+    float mx = of(0)[P::ML + r];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mx = fmaxf(mx, of(x)[P::ML + r]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float lt = 0.f;
+    floatx4 acc = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float wt = exp2_fast(of(x)[P::ML + r] - mu);
+      lt = fmaf(of(x)[P::ML + BR + r], wt, lt);
+      acc += wt * *reinterpret_cast<const floatx4*>(of(x) + r * P::OROW + d);
+    }
+    if (state) {
+      *reinterpret_cast<floatx4*>(state + r * a.dv + d) = acc;
+      if (d == 0) {
+        state[BR * a.dv + r] = mx;
+        state[BR * a.dv + BR + r] = lt;
+      }
+    } else {
+      const float inv = mx == -INFINITY ? 0.f : 1.f / lt;
+      *reinterpret_cast<uint2*>(out_at(r) + d) = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+    }
+  }
+}
+
+// Joins a row block's pieces: out = sum_p exp2(m_p - M) acc_p / sum_p exp2(m_p - M) l_p. Grid (row blocks, key / value
+// heads, BR / RW) x 256: RW rows to a workgroup, 256 / RW lanes to a row, of which dv / 4 read a piece's sums side by side.
+template <class T, int BR, int GR, int RW>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  constexpr int LANES = 256 / RW;
+  __shared__ float s_m[256], s_l[256];
+  __shared__ __align__(16) floatx4 s_acc[256];
+  const int tid = threadIdx.x, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
+  const Work w = scalars(find_work<BR, GR, true>(a, blockIdx.x));
+  if (w.b < 0 || w.s.kv < 0) return;
+  const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<GR>(keys, w.cut);
+  if (pieces == 1) return;  // written by the piece itself
+  const int n4 = a.dv / 4, r = static_cast<int>(blockIdx.z) * RW + tid / LANES, rows = min(BR, w.s.n * G - w.blk * BR);
+  const int t = tid % LANES, side = LANES / n4, p0 = t / n4, d = 4 * (t - p0 * n4);
+  const float* first = state_at<BR>(a, w.slot, kvh);
+  const int64_t step = static_cast<int64_t>(a.nkv) * BR * (a.dv + 2);
+  float m = -INFINITY, l = 0.f;
+  floatx4 acc = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (r < rows && p0 < side) {
+    constexpr int kAtOnce = 8;
+    for (int p = p0; p < pieces; p += side * kAtOnce) {
+      float pm[kAtOnce], pl[kAtOnce];
+      floatx4 pa[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const float* s = first + min(p + u * side, pieces - 1) * step;
+        pm[u] = s[BR * a.dv + r];
+        pl[u] = s[BR * a.dv + BR + r];
+        pa[u] = *reinterpret_cast<const floatx4*>(s + r * a.dv + d);
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) mn = fmaxf(mn, p + u * side < pieces ? pm[u] : -INFINITY);
+      const float mu = mn == -INFINITY ? 0.f : mn, alpha = exp2_fast(m - mu);
+      m = mn;
+      l *= alpha;
+      acc *= alpha;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (p + u * side < pieces) {
+          const float wt = exp2_fast(pm[u] - mu);
+          l = fmaf(pl[u], wt, l);
+          acc += wt * pa[u];
+        }
+    }
+  }
+  s_m[tid] = m;
+  s_l[tid] = l;
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (r >= rows || p0 != 0) return;
+  float mx = m;
+  for (int x = 1; x < side; ++x) mx = fmaxf(mx, s_m[tid + x * n4]);
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  float lt = 0.f;
+  floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int x = 0; x < side; ++x) {
+    const float wt = exp2_fast(s_m[tid + x * n4] - mu);
+    lt = fmaf(s_l[tid + x * n4], wt, lt);
+    sum += wt * s_acc[tid + x * n4];
+  }
+  const int row = w.blk * BR + r, i = static_cast<int>(div_by(row, a.group));
+  const float inv = mx == -INFINITY ? 0.f : 1.f / lt;
+  *reinterpret_cast<uint2*>(a.out.at(w.s.first + i, kvh * G + (row - i * G)) + d) =
+      make_uint2(pack2<T>(sum[0] * inv, sum[1] * inv), pack2<T>(sum[2] * inv, sum[3] * inv));
+}
+
+template <class T, int NW, int NKQ, int NT, bool PAGED>
+int launch_shape(const AttnArgs& a, const FewPlan& p, hipStream_t st, const char* what) {
+  using P = Few<1, NW, NKQ, NT>;
+  auto kern = few_kernel<T, 1, NW, NKQ, NT, PAGED>;
+  int rc = mm::allow_lds(kern, P::LDS, what);
+  if (rc) return rc;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(p.blocks + p.target), static_cast<unsigned>(a.nkv)), dim3(NW * kWave), P::LDS,
+                     st, a);
+  rc = mm::check_launch(what);
+  if (rc || p.target == 0) return rc;
+  constexpr int RW = 1;
+  hipLaunchKernelGGL((join_kernel<T, P::BR, P::GR, RW>),
+                     dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(a.nkv), P::BR / RW), dim3(256), 0, st, a);
+  return mm::check_launch(what);
+}
+
+template <class T, bool PAGED>
+int launch_type(const AttnArgs& a, const FewPlan& p, hipStream_t st, const char* what) {
+  if (a.dqk <= 64 && a.dv <= 64) return launch_shape<T, 8, 2, 4, PAGED>(a, p, st, what);
+  if (a.dqk <= 128 && a.dv <= 128) return launch_shape<T, 8, 4, 8, PAGED>(a, p, st, what);
+  if (a.dqk <= 192 && a.dv <= 128) return launch_shape<T, 8, 6, 8, PAGED>(a, p, st, what);
+  return launch_shape<T, 4, 8, 16, PAGED>(a, p, st, what);
+}
+
+}  // namespace
+
+FewPlan plan_few(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+  constexpr int64_t BR = 16;
+  const int64_t G = nh / nkv, rows = tokens * G, gr = (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys;
+  FewPlan p{};
+  p.blocks = rows / BR + seqs < rows ? rows / BR + seqs : rows;
+  if (max_keys > gr) p.target = (2 * mm::cu_count() + nkv - 1) / nkv;
+  p.workspace = 2 * p.target * nkv * BR * (dv + 2) * 4;
+  return p;
+}
+
+int launch_few(AttnArgs& a, const FewPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {
+  a.target = static_cast<int>(p.target);
+  if (dtype == MM_BF16)
+    return paged ? launch_type<BF16, true>(a, p, st, what) : launch_type<BF16, false>(a, p, st, what);
+  return paged ? launch_type<FP16, true>(a, p, st, what) : launch_type<FP16, false>(a, p, st, what);
+}
+
+}  // namespace mmp

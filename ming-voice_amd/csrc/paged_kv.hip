@@ -2,129 +2,14 @@
 // pages, and the attention over packed prompts (C ABI: mingpaged.h).
 //
 //   paged_append_kernel   rotation and stores, one pass over q, k and v
-//   attn_rows_kernel      attention, one wave per token and query head
+//   few_kernel            attention of few rows (paged_few.hip)
 #include <cmath>
 
-#include "mingpaged.h"
-#include "mm_common.h"
+#include "paged_common.h"
 
 namespace {
 
-using namespace mmd;
-
-// ------------------------------------------------------------------------------------------ shared pieces
-
-// n / d for n < 2^31 by a multiplication: m = floor(2^(31 + l) / d) + 1 with l = ceil(log2 d) exceeds 2^(31 + l) / d by at
-// most 1 <= 2^l / d, so the product is off by less than 1 / d for every such n.
-struct FastDiv {
-  uint32_t d, m;
-  int s;
-};
-
-FastDiv fast_div(int64_t d) {
-  FastDiv f{static_cast<uint32_t>(d), 0, 0};
-  if (d > 1) {
-    int l = 0;
-    while ((1LL << l) < d) ++l;
-    f.m = static_cast<uint32_t>((1ULL << (31 + l)) / static_cast<uint64_t>(d) + 1);
-    f.s = l - 1;
-  }
-  return f;
-}
-
-__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) {
-  return f.d == 1 ? n : __umulhi(n, f.m) >> f.s;
-}
-
-// The batch as the kernels see it: device arrays of one index type, every value clamped before use, so that no content of
-// them leads outside a buffer.
-struct Batch {
-  const void* cu;
-  const void* lens;
-  const void* table;
-  int64_t table_stride;
-  int i64;          // the arrays hold 64-bit numbers
-  int seqs, tokens;
-  int max_keys;     // max_pages * page
-};
-
-__device__ __forceinline__ int64_t idx_at(const void* p, int i64, int64_t i) {
-  return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
-}
-
-// A stream's first token, the number of its tokens and the rows of its cache that count (-1: outside the table).
-struct Stream {
-  int first, n, kv;
-};
-
-__device__ __forceinline__ Stream stream_at(const Batch& a, int b) {
-  const int64_t c0 = idx_at(a.cu, a.i64, b), c1 = idx_at(a.cu, a.i64, b + 1);
-  Stream s;
-  s.first = static_cast<int>(min(max(c0, static_cast<int64_t>(0)), static_cast<int64_t>(a.tokens)));
-  s.n = static_cast<int>(min(max(c1, static_cast<int64_t>(s.first)), static_cast<int64_t>(a.tokens))) - s.first;
-  if (a.lens) {
-    const int64_t kv = idx_at(a.lens, a.i64, b);
-    s.kv = kv < 0 || kv > a.max_keys ? -1 : static_cast<int>(kv);
-  } else {
-    s.kv = s.n;  // a prompt's own rows
-  }
-  return s;
-}
-
-// The stream that token t belongs to (seqs: none), found by the whole wave: the number of streams that end at or before t.
-__device__ __forceinline__ int stream_of_token(const Batch& a, int t) {
-  int b = 0;
-  for (int base = 0; base < a.seqs; base += kWave) {
-    const int i = base + lane_id();
-    const bool before = i < a.seqs && idx_at(a.cu, a.i64, min(i, a.seqs - 1) + 1) <= t;
-    const int n = __popcll(__ballot(before));
-    b += n;
-    if (n < kWave) break;
-  }
-  return min(b, a.seqs);
-}
-
-template <class T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (T::kBf16) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      x[2 * i] = f16_to_f32(static_cast<uint16_t>(w[i]));
-      x[2 * i + 1] = f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
-    }
-  }
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (T::kBf16) return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
-  else return static_cast<uint32_t>(f32_to_f16(lo)) | (static_cast<uint32_t>(f32_to_f16(hi)) << 16);
-}
-
-template <class T>
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-}
-
-__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
-__device__ __forceinline__ void st16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
-
-// Rows [tokens, heads, d] of a packed tensor, or one page's: element strides.
-struct Rows {
-  uint16_t* p;
-  int64_t ts, hs;
-  __device__ __forceinline__ uint16_t* at(int64_t t, int h) const { return p + t * ts + h * hs; }
-};
-
-struct Pool {
-  uint16_t* p;
-  int64_t ps, hs, rs;
-  __device__ __forceinline__ uint16_t* at(int64_t page, int h, int row) const { return p + page * ps + h * hs + row * rs; }
-};
+using namespace mmp;
 
 // ------------------------------------------------------------------------------------------ append
 
@@ -254,95 +139,6 @@ int launch_append(const AppendArgs& a, hipStream_t st) {
   return mm::check_launch("paged_append");
 }
 
-// ------------------------------------------------------------------------------------------ attention
-
-struct AttnArgs {
-  Rows q, out;
-  Rows k, v;    // a prompt's packed rows
-  Pool kp, vp;  // the cache
-  Batch batch;
-  FastDiv page, group;
-  int64_t n_pages;
-  int nh, nkv, dqk, dv;
-  float scale;
-};
-
-// One wave per token and query head: 64 keys at a time, a key to a lane for the scores, dims to the lanes for the values.
-template <class T, bool PAGED>
-__global__ __launch_bounds__(kWave) void attn_rows_kernel(AttnArgs a) {
-  __shared__ float s_q[256], s_p[kWave];
-  __shared__ const uint16_t* s_v[kWave];
-  const int t = blockIdx.x, h = blockIdx.y, lane = lane_id();
-  const int b = stream_of_token(a.batch, t);
-  if (b >= a.batch.seqs) return;
-  const Stream s = stream_at(a.batch, b);
-  uint16_t* o = a.out.at(t, h);
-  if (s.kv < 0) {
-    for (int d = lane; d < a.dv; d += kWave) T::st(o, d, NAN);
-    return;
-  }
-  const int kvh = static_cast<int>(div_by(h, a.group)), lim = s.kv - s.n + (t - s.first) + 1;
-  for (int d = lane; d < a.dqk; d += kWave) s_q[d] = T::ld(a.q.at(t, h), d);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < lim; k0 += kWave) {
-    const int key = k0 + lane;
-    const uint16_t *kr = nullptr, *vr = nullptr;
-    if (key < lim) {
-      if constexpr (PAGED) {
-        const int pg = static_cast<int>(div_by(key, a.page)), row = key - pg * static_cast<int>(a.page.d);
-        const int64_t id = idx_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + pg);
-        if (id >= 0 && id < a.n_pages) {
-          kr = a.kp.at(id, kvh, row);
-          vr = a.vp.at(id, kvh, row);
-        }
-      } else {
-        kr = a.k.at(s.first + key, kvh);
-        vr = a.v.at(s.first + key, kvh);
-      }
-    }
-    float sc = 0.f;
-    if (kr)
-      for (int d = 0; d < a.dqk; d += 8) {
-        float x[8];
-        unpack8<T>(ld16(kr + d), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sc = fmaf(x[e], s_q[d + e], sc);
-      }
-    sc = kr ? sc * a.scale : -INFINITY;
-    const float mn = fmaxf(m, wave_max(sc)), mu = mn == -INFINITY ? 0.f : mn;
-    const float p = kr ? expf(sc - mu) : 0.f, alpha = expf(m - mu);
-    m = mn;
-    l = fmaf(l, alpha, wave_sum(p));
-    __syncthreads();
-    s_p[lane] = p;
-    s_v[lane] = vr;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= alpha;
-    for (int j = 0; j < kWave; ++j) {
-      if (!s_v[j]) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = lane + kWave * e;
-        if (d < a.dv) acc[e] = fmaf(s_p[j], T::ld(s_v[j], d), acc[e]);
-      }
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + kWave * e;
-    if (d < a.dv) T::st(o, d, m == -INFINITY ? 0.f : acc[e] / l);
-  }
-}
-
-template <class T, bool PAGED>
-int launch_attn(const AttnArgs& a, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL((attn_rows_kernel<T, PAGED>), dim3(static_cast<unsigned>(a.batch.tokens), static_cast<unsigned>(a.nh)),
-                     dim3(kWave), 0, st, a);
-  return mm::check_launch(what);
-}
-
 // ------------------------------------------------------------------------------------------ checks on the host
 
 constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxKeys = (1LL << 31) - 1;
@@ -377,7 +173,8 @@ int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) 
   if (rc) return rc;
   if ((rc = check_tokens(what, b->tokens, b->seqs))) return rc;
   MM_REQUIRE(b->idx_dtype == MM_INT32 || b->idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
-  MM_REQUIRE(g->page >= 1 && g->n_pages >= 0 && b->max_pages >= 0 && b->table_stride >= 0, "%s: bad page or table sizes", what);
+  MM_REQUIRE(b->tokens * nh <= kMaxKeys, "%s: tokens * nh must be below 2^31", what);
+  MM_REQUIRE(g->page >= 1 && g->n_pages >= 0 && g->n_pages <= kMaxKeys && b->max_pages >= 0 && b->table_stride >= 0, "%s: bad page or table sizes", what);
   MM_REQUIRE(b->max_pages <= kMaxKeys / g->page, "%s: max_pages * page must be below 2^31", what);
   MM_REQUIRE(b->cu && b->kv_lens && (b->table || b->max_pages == 0), "%s: null batch array", what);
   MM_REQUIRE(g->n_pages == 0 || (g->k && g->v), "%s: null pool", what);
@@ -397,6 +194,24 @@ Rows rows_of(const void* p, int64_t ts, int64_t hs) { return Rows{static_cast<ui
 void set_pool(const mm_pages* g, Pool& k, Pool& v) {
   k = Pool{static_cast<uint16_t*>(g->k), g->k_page_stride, g->k_head_stride, g->k_row_stride};
   v = Pool{static_cast<uint16_t*>(g->v), g->v_page_stride, g->v_head_stride, g->v_row_stride};
+}
+
+int64_t workspace_of(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+  return plan_few(tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
+}
+
+int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int64_t workspace_bytes, hipStream_t st,
+           const char* what) {
+  const int64_t max_keys = paged ? a.batch.max_keys : a.batch.tokens;
+  // 0 would turn the -infinity of a key that is not seen into NaN; this leaves every finite score at zero
+  a.scale = scale == 0.f ? 1e-37f : fabsf(scale);
+  a.negative = scale < 0.f;
+  const FewPlan p = plan_few(a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
+  MM_REQUIRE(p.blocks + p.target <= 0x7fffffff, "%s: too many rows", what);
+  MM_REQUIRE(p.workspace == 0 || (workspace && mm::aligned16(workspace) && workspace_bytes >= p.workspace),
+             "%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)p.workspace);
+  a.ws = static_cast<float*>(workspace);
+  return launch_few(a, p, dtype, paged, st, what);
 }
 
 }  // namespace
@@ -449,7 +264,7 @@ extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t
   if (check_shape("paged_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("paged_attn", tokens, seqs) || max_keys < 0 ||
       max_keys > kMaxKeys)
     return -1;
-  return 0;
+  return workspace_of(tokens, seqs, max_keys, nh, nkv, dqk, dv);
 }
 
 extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
@@ -467,19 +282,17 @@ extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, 
   a.batch = batch_of(pages, batch);
   a.page = fast_div(pages->page);
   a.group = fast_div(nh / pages->nkv);
-  a.n_pages = pages->n_pages;
+  a.n_pages = static_cast<int>(pages->n_pages);
   a.nh = nh;
   a.nkv = pages->nkv;
   a.dqk = pages->dqk;
   a.dv = pages->dv;
-  a.scale = scale;
-  return pages->dtype == MM_BF16 ? launch_attn<BF16, true>(a, MM_STREAM(stream), what)
-                                 : launch_attn<FP16, true>(a, MM_STREAM(stream), what);
+  return attend(a, pages->dtype, true, scale, workspace, workspace_bytes, MM_STREAM(stream), what);
 }
 
 extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv) {
   if (check_shape("prompt_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("prompt_attn", tokens, seqs)) return -1;
-  return 0;
+  return workspace_of(tokens, seqs, tokens, nh, nkv, dqk, dv);
 }
 
 extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
@@ -492,6 +305,7 @@ extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const v
   if ((rc = check_tokens(what, tokens, seqs))) return rc;
   MM_REQUIRE(idx_dtype == MM_INT32 || idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
   MM_REQUIRE(cu, "%s: null cu", what);
+  MM_REQUIRE(tokens * nh <= kMaxKeys, "%s: tokens * nh must be below 2^31", what);
   if (tokens == 0 || seqs == 0) return MM_OK;
   if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "k", k, k_ts, k_hs, 16)) ||
       (rc = check_rows(what, "v", v, v_ts, v_hs, 16)) || (rc = check_rows(what, "out", out, o_ts, o_hs, 8)))
@@ -508,7 +322,5 @@ extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const v
   a.nkv = nkv;
   a.dqk = dqk;
   a.dv = dv;
-  a.scale = scale;
-  return dtype == MM_BF16 ? launch_attn<BF16, false>(a, MM_STREAM(stream), what)
-                          : launch_attn<FP16, false>(a, MM_STREAM(stream), what);
+  return attend(a, dtype, false, scale, workspace, workspace_bytes, MM_STREAM(stream), what);
 }

@@ -124,11 +124,11 @@ def test_attn_refuses():
     assert "null q" in err(attn(q=None)) and "null out" in err(attn(out=None))
     assert "strides of q" in err(attn(q_ts=892)) and "out must be 8-byte" in err(attn(out=P + 4))
     assert "strides of out" in err(attn(o_hs=66))
-    need = mm.load().mm_paged_attn_workspace(5, 3, 64, 14, 2, 64, 64)
-    assert need >= 0
-    if need:
-        assert "workspace" in err(attn(ws_bytes=need - 1)) and "workspace" in err(attn(ws=None))
-        assert "workspace" in err(attn(ws=P + 4))
+    assert "tokens * nh" in err(attn(b=batch(tokens=1 << 22), nh=512))
+    need = mm.load().mm_paged_attn_workspace(5, 3, 16 * 1000, 14, 2, 64, 64)  # a table that allows long contexts
+    long = batch(max_pages=1000, table_stride=1000)
+    assert need > 0 and "workspace" in err(attn(b=long, ws_bytes=need - 1)) and "workspace" in err(attn(b=long, ws=None))
+    assert "workspace" in err(attn(b=long, ws=P + 4))
 
 
 def test_prompt_refuses():
