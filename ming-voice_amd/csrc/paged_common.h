@@ -282,6 +282,11 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
   return (w & lo) == lo || (w & hi) == hi;
 }
 
+template <class T>
+__device__ __forceinline__ float value_of(uint32_t bits) {  // of the low half
+  return T::kBf16 ? __uint_as_float(bits << 16) : f16_to_f32(static_cast<uint16_t>(bits));
+}
+
 // The page number read for a key, as it came (both halves of a 64-bit entry; the same word twice of a 32-bit one), so
 // that nothing waits for it before it is used.
 struct PageId {
@@ -301,11 +306,15 @@ __device__ __forceinline__ bool page_ok(const AttnArgs& a, PageId id) {
 // What a row that does not exist reads.
 static __device__ const uint4 kZeroRow[32] = {};
 
-// The attention of blocks of few rows (16), whose waves share out the keys.
-struct FewPlan {
+// What a call launches. Few rows to a block (16) or many (128); target: pieces of keys aimed at for the whole batch (0: no
+// cutting, no join); blocks: the most row blocks that these sizes can have.
+struct AttnPlan {
+  bool many;
   int64_t blocks, target, workspace;
 };
-FewPlan plan_few(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
-int launch_few(AttnArgs& a, const FewPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
+AttnPlan plan_attn(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
+int launch_many(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
+int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what);
 
 }  // namespace mmp

@@ -25,8 +25,8 @@ struct Few {
   static_assert(LDS <= 160 * 1024 && KI % 2 == 0 && NT % 4 == 0, "tile shape");
 };
 
-// Softmax attention of up to 16 QF rows over a piece of their keys, one pass with a running maximum and sum. Grid (work,
-// key / value heads) x NW waves. Wave w takes tiles w, w + NW, ... of 32 keys of the piece; the waves' states meet in LDS.
+// Softmax attention of up to 16 QF rows over a piece of their keys, one pass with a running maximum and sum. Grid (work x key /
+// value heads) x NW waves. Wave w takes tiles w, w + NW, ... of 32 keys of the piece; the waves' states meet in LDS.
 // Per tile, on the 16x16x32 MFMA (bf16 or fp16, fp32 sums):
 //   S^T [32 keys, 16 rows] = K Q^T: the key rows as A fragments from LDS, the rows' queries held as B fragments;
 //   the softmax update per row is lane-local (a lane of S^T holds 8 keys of row lane % 16), the maximum over 4 lanes;
@@ -36,7 +36,7 @@ struct Few {
 // requested as soon as this one's are in registers, its values as soon as this one's are; the page numbers of the tile
 // after that are read one tile ahead, lane l for key l % 32, and handed to the loading lanes by ds_bpermute. Keys that no
 // row sees (past the piece, in a missing page) read a row of zeros. A value that some rows must not see could still be an
-// infinity or NaN (0 * inf): such tiles take their values key by key (spill_safe below).
+// infinity or NaN (0 * inf): such tiles take their values key by key.
 template <class T, int QF, int NW, int NKQ, int NT, bool PAGED>
 __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   using P = Few<QF, NW, NKQ, NT>;
@@ -44,8 +44,9 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   extern __shared__ __align__(16) char s_few[];
   const int tid = threadIdx.x, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int lr = lane & 15, lq = lane >> 4, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
-  const Work w = scalars(find_work<BR, P::GR, false>(a, blockIdx.x));
+  const int lr = lane & 15, lq = lane >> 4, G = static_cast<int>(a.group.d);
+  const int unit = static_cast<int>(blockIdx.x) / a.nkv, kvh = static_cast<int>(blockIdx.x) - unit * a.nkv;
+  const Work w = scalars(find_work<BR, P::GR, false>(a, unit));
   if (w.b < 0) return;
   const int r0 = w.blk * BR, rows = min(BR, w.s.n * G - r0), n4 = a.dv / 4;
   auto out_at = [&](int r) {  // row r0 + r of the stream
@@ -246,16 +247,15 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
                 const uint32_t pw = e < 2 ? w0 : e < 4 ? w1 : e < 6 ? w2 : w3;
                 const uint32_t pk = static_cast<uint32_t>(
                     __builtin_amdgcn_ds_bpermute(4 * (lr + 16 * (key % 16 / 4)), static_cast<int>(pw)));
-                const uint16_t pb = static_cast<uint16_t>(e & 1 ? pk >> 16 : pk);
-                const float p = T::kBf16 ? bf16_to_f32(pb) : f16_to_f32(pb);
+                const uint32_t see = (sees[f] >> key) & 1u ? ~0u : 0u;
+                const float p = value_of<T>((e & 1 ? pk >> 16 : pk) & see);
                 const int d = 16 * (n0 + b) + 4 * lq;
-                const uint16_t* v = reinterpret_cast<const uint16_t*>(vt + key * P::VC * 16 +
-                                                                      v_chunk_at<P::VC>(key, d / 8) * 16) + d % 8;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const float x = T::kBf16 ? bf16_to_f32(v[j]) : f16_to_f32(v[j]);
-                  o[f][n0 + b][j] = (sees[f] >> key) & 1u ? fmaf(p, x, o[f][n0 + b][j]) : o[f][n0 + b][j];
-                }
+                const uint2 x = *reinterpret_cast<const uint2*>(vt + key * P::VC * 16 + v_chunk_at<P::VC>(key, d / 8) * 16 + (d % 8) * 2);
+                floatx4& ob = o[f][n0 + b];
+                ob[0] = fmaf(p, value_of<T>(x.x & see), ob[0]);
+                ob[1] = fmaf(p, value_of<T>((x.x & see) >> 16), ob[1]);
+                ob[2] = fmaf(p, value_of<T>(x.y & see), ob[2]);
+                ob[3] = fmaf(p, value_of<T>((x.y & see) >> 16), ob[3]);
               }
             }
             continue;
@@ -380,24 +380,26 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
       make_uint2(pack2<T>(sum[0] * inv, sum[1] * inv), pack2<T>(sum[2] * inv, sum[3] * inv));
 }
 
+template <class T, int BR, int GR, int RW>
+int launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
+  hipLaunchKernelGGL((join_kernel<T, BR, GR, RW>),
+                     dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(a.nkv), BR / RW), dim3(256), 0, st, a);
+  return mm::check_launch(what);
+}
+
 template <class T, int NW, int NKQ, int NT, bool PAGED>
-int launch_shape(const AttnArgs& a, const FewPlan& p, hipStream_t st, const char* what) {
+int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
   using P = Few<1, NW, NKQ, NT>;
   auto kern = few_kernel<T, 1, NW, NKQ, NT, PAGED>;
   int rc = mm::allow_lds(kern, P::LDS, what);
   if (rc) return rc;
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(p.blocks + p.target), static_cast<unsigned>(a.nkv)), dim3(NW * kWave), P::LDS,
-                     st, a);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)), dim3(NW * kWave), P::LDS, st, a);
   rc = mm::check_launch(what);
-  if (rc || p.target == 0) return rc;
-  constexpr int RW = 1;
-  hipLaunchKernelGGL((join_kernel<T, P::BR, P::GR, RW>),
-                     dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(a.nkv), P::BR / RW), dim3(256), 0, st, a);
-  return mm::check_launch(what);
+  return rc || p.target == 0 ? rc : launch_join<T, P::BR, P::GR, 1>(a, p, st, what);
 }
 
 template <class T, bool PAGED>
-int launch_type(const AttnArgs& a, const FewPlan& p, hipStream_t st, const char* what) {
+int launch_type(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
   if (a.dqk <= 64 && a.dv <= 64) return launch_shape<T, 8, 2, 4, PAGED>(a, p, st, what);
   if (a.dqk <= 128 && a.dv <= 128) return launch_shape<T, 8, 4, 8, PAGED>(a, p, st, what);
   if (a.dqk <= 192 && a.dv <= 128) return launch_shape<T, 8, 6, 8, PAGED>(a, p, st, what);
@@ -406,21 +408,25 @@ int launch_type(const AttnArgs& a, const FewPlan& p, hipStream_t st, const char*
 
 }  // namespace
 
-FewPlan plan_few(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
-  constexpr int64_t BR = 16;
-  const int64_t G = nh / nkv, rows = tokens * G, gr = (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys;
-  FewPlan p{};
-  p.blocks = rows / BR + seqs < rows ? rows / BR + seqs : rows;
+AttnPlan plan_attn(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+  AttnPlan p{};
+  const int64_t rows = tokens * (nh / nkv);
+  p.many = rows > 16 * seqs;  // more than 16 rows a stream on average
+  const int64_t br = p.many ? 128 : 16, gr = p.many ? 64 : (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys;
+  p.blocks = rows / br + seqs < rows ? rows / br + seqs : rows;
   if (max_keys > gr) p.target = (2 * mm::cu_count() + nkv - 1) / nkv;
-  p.workspace = 2 * p.target * nkv * BR * (dv + 2) * 4;
+  p.workspace = 2 * p.target * nkv * br * (dv + 2) * 4;
   return p;
 }
 
-int launch_few(AttnArgs& a, const FewPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {
-  a.target = static_cast<int>(p.target);
+int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {
   if (dtype == MM_BF16)
     return paged ? launch_type<BF16, true>(a, p, st, what) : launch_type<BF16, false>(a, p, st, what);
   return paged ? launch_type<FP16, true>(a, p, st, what) : launch_type<FP16, false>(a, p, st, what);
+}
+
+int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what) {
+  return dtype == MM_BF16 ? launch_join<BF16, 128, 64, 4>(a, p, st, what) : launch_join<FP16, 128, 64, 4>(a, p, st, what);
 }
 
 }  // namespace mmp

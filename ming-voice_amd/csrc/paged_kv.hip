@@ -2,7 +2,8 @@
 // pages, and the attention over packed prompts (C ABI: mingpaged.h).
 //
 //   paged_append_kernel   rotation and stores, one pass over q, k and v
-//   few_kernel            attention of few rows (paged_few.hip)
+//   few_kernel            attention of few rows, join_kernel (paged_few.hip)
+//   many_kernel           attention of many rows (paged_many.hip)
 #include <cmath>
 
 #include "paged_common.h"
@@ -197,7 +198,7 @@ void set_pool(const mm_pages* g, Pool& k, Pool& v) {
 }
 
 int64_t workspace_of(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
-  return plan_few(tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
+  return plan_attn(tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
 }
 
 int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int64_t workspace_bytes, hipStream_t st,
@@ -206,12 +207,13 @@ int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int
   // 0 would turn the -infinity of a key that is not seen into NaN; this leaves every finite score at zero
   a.scale = scale == 0.f ? 1e-37f : fabsf(scale);
   a.negative = scale < 0.f;
-  const FewPlan p = plan_few(a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
-  MM_REQUIRE(p.blocks + p.target <= 0x7fffffff, "%s: too many rows", what);
+  const AttnPlan p = plan_attn(a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
+  MM_REQUIRE((p.blocks + p.target) * a.nkv <= 0x7fffffff, "%s: too many rows", what);
   MM_REQUIRE(p.workspace == 0 || (workspace && mm::aligned16(workspace) && workspace_bytes >= p.workspace),
              "%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)p.workspace);
   a.ws = static_cast<float*>(workspace);
-  return launch_few(a, p, dtype, paged, st, what);
+  a.target = static_cast<int>(p.target);
+  return p.many ? launch_many(a, p, dtype, paged, st, what) : launch_few(a, p, dtype, paged, st, what);
 }
 
 }  // namespace
