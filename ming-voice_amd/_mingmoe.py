@@ -50,12 +50,14 @@ class Pages(ctypes.Structure):
                 ("dv", ctypes.c_int32), ("n_pages", _I64), ("page", _I64), ("k_page_stride", _I64),
                 ("k_head_stride", _I64), ("k_row_stride", _I64), ("v_page_stride", _I64), ("v_head_stride", _I64),
                 ("v_row_stride", _I64)]
+    _as_parameter_ = property(ctypes.byref)
 
 
 class Batch(ctypes.Structure):
     """mm_batch: packed tokens of several streams (cu, kv_lens and the page table, device arrays of one dtype)."""
     _fields_ = [("cu", _P), ("kv_lens", _P), ("table", _P), ("table_stride", _I64), ("max_pages", _I64),
                 ("seqs", _I64), ("tokens", _I64), ("idx_dtype", ctypes.c_int32)]
+    _as_parameter_ = property(ctypes.byref)
 
 
 SIGNATURES = {
@@ -120,10 +122,9 @@ SIGNATURES = {
 PAGED_VERSION = 1
 PAGED_SIGNATURES = {
     "mm_paged_version": ([], ctypes.c_int),
-    "mm_paged_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, ctypes.POINTER(Pages),
-                         ctypes.POINTER(Batch), _P, _I64, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P], ctypes.c_int),
+    "mm_paged_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P], ctypes.c_int),
     "mm_paged_attn_workspace": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
-    "mm_paged_attn": ([_P, _I64, _I64, _I32, ctypes.POINTER(Pages), ctypes.POINTER(Batch), _F32, _P, _I64, _I64, _P,
+    "mm_paged_attn": ([_P, _I64, _I64, _I32, _P, _P, _F32, _P, _I64, _I64, _P,
                        _I64, _P], ctypes.c_int),
     "mm_prompt_attn_workspace": ([_I64, _I64, _I32, _I32, _I32, _I32], _I64),
     "mm_prompt_attn": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64,

@@ -185,9 +185,9 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
   return v;
 }
 
-// The work of workgroup w (BY_BLOCK: of row block w, piece 0), found by every wave from the batch itself: streams 64 at a
+// The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the batch itself: streams 64 at a
 // time, one to a lane. Within a stream the last row block, whose rows see the most keys, comes first.
-template <int BR, int GR, bool BY_BLOCK>
+template <int BR, int GR, bool CUT>
 __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
   const int G = static_cast<int>(a.group.d), lane = lane_id(), B = a.batch.seqs;
   Work k{-1, 0, 0, 0, 0, Stream{0, 0, 0}};
@@ -211,19 +211,19 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
   for (int base = 0; base < B; base += kWave) {
     if (base) load(base);
     const int blocks = blocks_of<BR>(mine, G), pieces = pieces_of<GR>(max(mine.kv, 0), k.cut);
-    const int units = BY_BLOCK ? blocks : blocks * pieces, held = pieces > 1 ? blocks * pieces : 0;
+    const int held = pieces > 1 ? blocks * pieces : 0, units = !CUT ? blocks * pieces : held ? blocks : 0;
     const int ends = wave_scan(units), last = __builtin_amdgcn_readlane(ends, kWave - 1);
     if (w < last) {
       const int src = __ffsll(static_cast<long long>(__ballot(ends > w))) - 1;
       const int held_before = wave_scan(held) - held;
       const int u = w - (__builtin_amdgcn_readlane(ends, src) - __builtin_amdgcn_readlane(units, src));
       const int p = __builtin_amdgcn_readlane(pieces, src), nb = __builtin_amdgcn_readlane(blocks, src);
-      const int at = BY_BLOCK ? u : u / p;
+      const int at = CUT ? u : u / p;
       k.b = base + src;
       k.s = Stream{__builtin_amdgcn_readlane(mine.first, src), __builtin_amdgcn_readlane(mine.n, src),
                    __builtin_amdgcn_readlane(mine.kv, src)};
       k.blk = nb - 1 - at;
-      k.piece = BY_BLOCK ? 0 : u - at * p;
+      k.piece = CUT ? 0 : u - at * p;
       k.slot = slots + __builtin_amdgcn_readlane(held_before, src) + at * p;
       // always so for a cu that does not fall; one that does must not lead out of the buffers either
       if (u < 0 || at >= nb || (p > 1 && (k.slot < 0 || k.slot + p > 2 * a.target))) k.b = -1;

@@ -313,77 +313,84 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   }
 }
 
-// Joins a row block's pieces: out = sum_p exp2(m_p - M) acc_p / sum_p exp2(m_p - M) l_p. Grid (row blocks, key / value
-// heads, BR / RW) x 256: RW rows to a workgroup, 256 / RW lanes to a row, of which dv / 4 read a piece's sums side by side.
-template <class T, int BR, int GR, int RW>
+// Joins the pieces of a row block that was cut: out = sum_p exp2(m_p - M) acc_p / sum_p exp2(m_p - M) l_p. Grid (cut
+// blocks, key / value heads, BR / ROWS) x 256: RW rows at a time, 256 / RW lanes to a row, of which dv / 4 read a piece's
+// sums side by side and the rest other pieces'.
+template <class T, int BR, int GR, int ROWS, int RW>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   constexpr int LANES = 256 / RW;
   __shared__ float s_m[256], s_l[256];
   __shared__ __align__(16) floatx4 s_acc[256];
   const int tid = threadIdx.x, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
   const Work w = scalars(find_work<BR, GR, true>(a, blockIdx.x));
-  if (w.b < 0 || w.s.kv < 0) return;
+  if (w.b < 0) return;
   const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<GR>(keys, w.cut);
-  if (pieces == 1) return;  // written by the piece itself
-  const int n4 = a.dv / 4, r = static_cast<int>(blockIdx.z) * RW + tid / LANES, rows = min(BR, w.s.n * G - w.blk * BR);
+  if (pieces == 1) return;  // a block of few keys in a stream that is cut: written by the piece itself
+  const int n4 = a.dv / 4, rows = min(BR, w.s.n * G - w.blk * BR);
   const int t = tid % LANES, side = LANES / n4, p0 = t / n4, d = 4 * (t - p0 * n4);
   const float* first = state_at<BR>(a, w.slot, kvh);
   const int64_t step = static_cast<int64_t>(a.nkv) * BR * (a.dv + 2);
-  float m = -INFINITY, l = 0.f;
-  floatx4 acc = floatx4{0.f, 0.f, 0.f, 0.f};
-  if (r < rows && p0 < side) {
-    constexpr int kAtOnce = 8;
-    for (int p = p0; p < pieces; p += side * kAtOnce) {
-      float pm[kAtOnce], pl[kAtOnce];
-      floatx4 pa[kAtOnce];
+  const int end = min(rows, static_cast<int>(blockIdx.z) * ROWS + ROWS);
+  for (int r0 = static_cast<int>(blockIdx.z) * ROWS; r0 < end; r0 += RW) {
+    const int r = r0 + tid / LANES;
+    float m = -INFINITY, l = 0.f;
+    floatx4 acc = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (r < end && p0 < side) {
+      constexpr int kAtOnce = 8;
+      for (int p = p0; p < pieces; p += side * kAtOnce) {
+        float pm[kAtOnce], pl[kAtOnce];
+        floatx4 pa[kAtOnce];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const float* s = first + min(p + u * side, pieces - 1) * step;
-        pm[u] = s[BR * a.dv + r];
-        pl[u] = s[BR * a.dv + BR + r];
-        pa[u] = *reinterpret_cast<const floatx4*>(s + r * a.dv + d);
-      }
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) mn = fmaxf(mn, p + u * side < pieces ? pm[u] : -INFINITY);
-      const float mu = mn == -INFINITY ? 0.f : mn, alpha = exp2_fast(m - mu);
-      m = mn;
-      l *= alpha;
-      acc *= alpha;
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u)
-        if (p + u * side < pieces) {
-          const float wt = exp2_fast(pm[u] - mu);
-          l = fmaf(pl[u], wt, l);
-          acc += wt * pa[u];
+        for (int u = 0; u < kAtOnce; ++u) {
+          const float* s = first + min(p + u * side, pieces - 1) * step;
+          pm[u] = s[BR * a.dv + r];
+          pl[u] = s[BR * a.dv + BR + r];
+          pa[u] = *reinterpret_cast<const floatx4*>(s + r * a.dv + d);
         }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) mn = fmaxf(mn, p + u * side < pieces ? pm[u] : -INFINITY);
+        const float mu = mn == -INFINITY ? 0.f : mn, alpha = exp2_fast(m - mu);
+        m = mn;
+        l *= alpha;
+        acc *= alpha;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (p + u * side < pieces) {
+            const float wt = exp2_fast(pm[u] - mu);
+            l = fmaf(pl[u], wt, l);
+            acc += wt * pa[u];
+          }
+      }
     }
+    __syncthreads();  // the last rows' values have been read
+    s_m[tid] = m;
+    s_l[tid] = l;
+    s_acc[tid] = acc;
+    __syncthreads();
+    if (r >= end || p0 != 0) continue;
+    float mx = m;
+    for (int x = 1; x < side; ++x) mx = fmaxf(mx, s_m[tid + x * n4]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float lt = 0.f;
+    floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < side; ++x) {
+      const float wt = exp2_fast(s_m[tid + x * n4] - mu);
+      lt = fmaf(s_l[tid + x * n4], wt, lt);
+      sum += wt * s_acc[tid + x * n4];
+    }
+    const int row = w.blk * BR + r, i = static_cast<int>(div_by(row, a.group));
+    const float inv = mx == -INFINITY ? 0.f : 1.f / lt;
+    *reinterpret_cast<uint2*>(a.out.at(w.s.first + i, kvh * G + (row - i * G)) + d) =
+        make_uint2(pack2<T>(sum[0] * inv, sum[1] * inv), pack2<T>(sum[2] * inv, sum[3] * inv));
   }
-  s_m[tid] = m;
-  s_l[tid] = l;
-  s_acc[tid] = acc;
-  __syncthreads();
-  if (r >= rows || p0 != 0) return;
-  float mx = m;
-  for (int x = 1; x < side; ++x) mx = fmaxf(mx, s_m[tid + x * n4]);
-  const float mu = mx == -INFINITY ? 0.f : mx;
-  float lt = 0.f;
-  floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int x = 0; x < side; ++x) {
-    const float wt = exp2_fast(s_m[tid + x * n4] - mu);
-    lt = fmaf(s_l[tid + x * n4], wt, lt);
-    sum += wt * s_acc[tid + x * n4];
-  }
-  const int row = w.blk * BR + r, i = static_cast<int>(div_by(row, a.group));
-  const float inv = mx == -INFINITY ? 0.f : 1.f / lt;
-  *reinterpret_cast<uint2*>(a.out.at(w.s.first + i, kvh * G + (row - i * G)) + d) =
-      make_uint2(pack2<T>(sum[0] * inv, sum[1] * inv), pack2<T>(sum[2] * inv, sum[3] * inv));
 }
 
-template <class T, int BR, int GR, int RW>
+template <class T, int BR, int GR, int ROWS, int RW>
 int launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL((join_kernel<T, BR, GR, RW>),
-                     dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(a.nkv), BR / RW), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((join_kernel<T, BR, GR, ROWS, RW>),
+                     dim3(static_cast<unsigned>(p.blocks < p.target ? p.blocks : p.target), static_cast<unsigned>(a.nkv), BR / ROWS),
+                     dim3(256), 0, st, a);
   return mm::check_launch(what);
 }
 
@@ -395,7 +402,7 @@ int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const cha
   if (rc) return rc;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)), dim3(NW * kWave), P::LDS, st, a);
   rc = mm::check_launch(what);
-  return rc || p.target == 0 ? rc : launch_join<T, P::BR, P::GR, 1>(a, p, st, what);
+  return rc || p.target == 0 ? rc : launch_join<T, P::BR, P::GR, 4, 4>(a, p, st, what);
 }
 
 template <class T, bool PAGED>
@@ -426,7 +433,7 @@ int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipS
 }
 
 int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what) {
-  return dtype == MM_BF16 ? launch_join<BF16, 128, 64, 4>(a, p, st, what) : launch_join<FP16, 128, 64, 4>(a, p, st, what);
+  return dtype == MM_BF16 ? launch_join<BF16, 128, 64, 32, 4>(a, p, st, what) : launch_join<FP16, 128, 64, 32, 4>(a, p, st, what);
 }
 
 }  // namespace mmp

@@ -144,11 +144,12 @@ int launch_append(const AppendArgs& a, hipStream_t st) {
 
 constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxKeys = (1LL << 31) - 1;
 
-int check_rows(const char* what, const char* name, const void* p, int64_t ts, int64_t hs, int align) {
+// A row of strides; those of a dim of one are not used and may be anything.
+int check_rows(const char* what, const char* name, const void* p, int64_t tokens, int64_t ts, int heads, int64_t hs, int align) {
   MM_REQUIRE(p, "%s: null %s", what, name);
   MM_REQUIRE((reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(align - 1)) == 0, "%s: %s must be %d-byte aligned",
              what, name, align);
-  MM_REQUIRE(ts >= 0 && hs >= 0 && ts % (align / 2) == 0 && hs % (align / 2) == 0,
+  MM_REQUIRE((tokens == 1 || (ts >= 0 && ts % (align / 2) == 0)) && (heads == 1 || (hs >= 0 && hs % (align / 2) == 0)),
              "%s: strides of %s must keep rows %d-byte aligned", what, name, align);
   return MM_OK;
 }
@@ -181,7 +182,9 @@ int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) 
   MM_REQUIRE(g->n_pages == 0 || (g->k && g->v), "%s: null pool", what);
   MM_REQUIRE(mm::aligned16(g->k) && mm::aligned16(g->v), "%s: the pool must be 16-byte aligned", what);
   const int64_t st[6] = {g->k_page_stride, g->k_head_stride, g->k_row_stride, g->v_page_stride, g->v_head_stride, g->v_row_stride};
-  for (int64_t s : st) MM_REQUIRE(s >= 0 && s % 8 == 0, "%s: the pool's strides must be multiples of 8", what);
+  const int64_t dims[3] = {g->n_pages, g->nkv, g->page};
+  for (int i = 0; i < 6; ++i)
+    MM_REQUIRE(dims[i % 3] <= 1 || (st[i] >= 0 && st[i] % 8 == 0), "%s: the pool's strides must be multiples of 8", what);
   return MM_OK;
 }
 
@@ -233,11 +236,14 @@ extern "C" int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const 
                  rot_offset + 2 * pairs <= pages->dqk,
              "paged_append: %lld pairs from dim %d on do not fit a head of %d (multiples of 8)", (long long)pairs, rot_offset,
              pages->dqk);
-  if (batch->tokens == 0 || batch->seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "k", k, k_ts, k_hs, 16)) ||
-      (rc = check_rows(what, "v", v, v_ts, v_hs, 16)) || (rc = check_rows(what, "q_out", q_out, qo_ts, qo_hs, 16)))
+  const int64_t N = batch->tokens;
+  const int nkv = pages->nkv;
+  if (N == 0 || batch->seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", q, N, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "k", k, N, k_ts, nkv, k_hs, 16)) ||
+      (rc = check_rows(what, "v", v, N, v_ts, nkv, v_hs, 16)) ||
+      (rc = check_rows(what, "q_out", q_out, N, qo_ts, nh, qo_hs, 16)))
     return rc;
-  if (k_out && (rc = check_rows(what, "k_out", k_out, ko_ts, ko_hs, 16))) return rc;
+  if (k_out && (rc = check_rows(what, "k_out", k_out, N, ko_ts, nkv, ko_hs, 16))) return rc;
   AppendArgs a{};
   a.q = rows_of(q, q_ts, q_hs);
   a.k = rows_of(k, k_ts, k_hs);
@@ -250,7 +256,7 @@ extern "C" int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const 
   a.n_pages = pages->n_pages;
   a.inv_freq = inv_freq;
   a.nh = nh;
-  a.nkv = pages->nkv;
+  a.nkv = nkv;
   a.dqk = pages->dqk;
   a.dv = pages->dv;
   a.pairs = static_cast<int>(pairs);
@@ -275,8 +281,9 @@ extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, 
   const char* what = "paged_attn";
   int rc = check_paged(what, nh, pages, batch);
   if (rc) return rc;
-  if (batch->tokens == 0 || batch->seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "out", out, o_ts, o_hs, 8))) return rc;
+  const int64_t N = batch->tokens;
+  if (N == 0 || batch->seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", q, N, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "out", out, N, o_ts, nh, o_hs, 8))) return rc;
   AttnArgs a{};
   a.q = rows_of(q, q_ts, q_hs);
   a.out = rows_of(out, o_ts, o_hs);
@@ -309,8 +316,8 @@ extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const v
   MM_REQUIRE(cu, "%s: null cu", what);
   MM_REQUIRE(tokens * nh <= kMaxKeys, "%s: tokens * nh must be below 2^31", what);
   if (tokens == 0 || seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, q_ts, q_hs, 16)) || (rc = check_rows(what, "k", k, k_ts, k_hs, 16)) ||
-      (rc = check_rows(what, "v", v, v_ts, v_hs, 16)) || (rc = check_rows(what, "out", out, o_ts, o_hs, 8)))
+  if ((rc = check_rows(what, "q", q, tokens, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "k", k, tokens, k_ts, nkv, k_hs, 16)) ||
+      (rc = check_rows(what, "v", v, tokens, v_ts, nkv, v_hs, 16)) || (rc = check_rows(what, "out", out, tokens, o_ts, nh, o_hs, 8)))
     return rc;
   AttnArgs a{};
   a.q = rows_of(q, q_ts, q_hs);

@@ -21,56 +21,103 @@ and for prompts that start from nothing prompt_attn(q, k, v, cu_seqlens) with th
 call's place. Every call enqueues on torch's current stream of its tensors' device and can be captured in a hipGraph;
 there is no CPU path.
 """
+import struct
+
 import torch
 
 import _mingmoe as _mm
 
 __all__ = ["paged_append", "paged_attn", "paged_attn_workspace", "prompt_attn", "prompt_attn_workspace"]
 
-
-def _rows(t, name, what, heads=None, width=None, dtype=None):
-    """(pointer, token stride, head stride) of a [tokens, heads, width] tensor with a contiguous last dim; the stride of a
-    dim of one is any number in torch and 0 here."""
-    if t.dim() != 3 or t.stride(2) != 1 or (heads is not None and t.shape[1] != heads) or \
-            (width is not None and t.shape[2] != width):
-        raise ValueError(f"{what}: {name} must be [tokens, {heads or 'heads'}, {width or 'd'}] with a contiguous last dim "
-                         f"(got {tuple(t.shape)}, strides {t.stride()})")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{what}: {name} must be {dtype} (got {t.dtype})")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+# mm_pages and mm_batch as bytes, and the current stream by its raw handle: a decode step calls these wrappers once a layer,
+# and building ctypes structures and stream objects took longer than the kernels (a call of paged_append 19.6 -> HOST us)
+_PAGES = struct.Struct("@2P4i8q")
+_BATCH = struct.Struct("@3P4qi4x")
+_HALF = (torch.bfloat16, torch.float16)
+_CODES = {torch.bfloat16: _mm.MM_BF16, torch.float16: _mm.MM_FP16, torch.int32: _mm.MM_INT32, torch.int64: _mm.MM_INT64}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _pages(k_pages, v_pages, what):
-    if k_pages.dim() != 4 or v_pages.dim() != 4 or k_pages.shape[:3] != v_pages.shape[:3] or k_pages.stride(3) != 1 or \
-            v_pages.stride(3) != 1:
-        raise ValueError(f"{what}: k_pages and v_pages must be [n_pages, nkv, page, d] with one n_pages, nkv and page and "
-                         f"contiguous rows (got {tuple(k_pages.shape)}, {tuple(v_pages.shape)})")
-    if k_pages.dtype != v_pages.dtype or k_pages.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{what}: k_pages and v_pages must both be bf16 or fp16 (got {k_pages.dtype}, {v_pages.dtype})")
+def _device(what, *tensors):
+    """The index of the GPU that holds every tensor."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            _mm.require_gpu(*tensors)
+    return dev
+
+
+def _rows(what, name, t, shape, dtype):
+    """(pointer, token stride, head stride) of a [tokens, heads, width] tensor with a contiguous last dim."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not dtype or s[-1] != 1:
+        raise ValueError(f"{what}: {name} must be a {dtype} {list(shape)} tensor with a contiguous last dim (got {t.dtype} "
+                         f"{list(t.shape)}, strides {s})")
+    return t.data_ptr(), s[0], s[1]
+
+
+def _queries(what, q, width, dtype):
+    """(tokens, heads, pointer, token stride, head stride) of q."""
+    shape, s = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != width or q.dtype is not dtype or s[2] != 1:
+        raise ValueError(f"{what}: q must be a {dtype} [tokens, heads, {width}] tensor with a contiguous last dim (got "
+                         f"{q.dtype} {list(shape)}, strides {s})")
+    return shape[0], shape[1], q.data_ptr(), s[0], s[1]
+
+
+def _pool(what, k_pages, v_pages):
+    """(mm_pages, n_pages, nkv, page, dqk, dv, dtype) of the pool."""
+    dt = k_pages.dtype
+    if k_pages.dim() != 4 or v_pages.dim() != 4 or v_pages.dtype is not dt or dt not in _HALF:
+        raise ValueError(f"{what}: k_pages and v_pages must both be bf16 or fp16 [n_pages, nkv, page, d] (got {k_pages.dtype} "
+                         f"{list(k_pages.shape)}, {v_pages.dtype} {list(v_pages.shape)})")
     n, nkv, page, dqk = k_pages.shape
-    ks, vs = ([s if m > 1 else 0 for s, m in zip(t.stride(), t.shape)] for t in (k_pages, v_pages))
-    return _mm.Pages(k_pages.data_ptr(), v_pages.data_ptr(), _mm.dtype_code(k_pages), nkv, dqk, v_pages.shape[3], n, page,
-                     ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    m, vkv, vpage, dv = v_pages.shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if n != m or nkv != vkv or page != vpage or k3 != 1 or v3 != 1:
+        raise ValueError(f"{what}: k_pages and v_pages must be [n_pages, nkv, page, d] with one n_pages, nkv and page and "
+                         f"contiguous rows (got {list(k_pages.shape)}, {list(v_pages.shape)})")
+    return (_PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), _CODES[dt], nkv, dqk, dv, n, page, k0, k1, k2, v0, v1, v2),
+            nkv, page, dqk, dv, dt)
 
 
-def _cu(cu_seqlens, what):
-    if cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] < 1 or \
-            cu_seqlens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: cu_seqlens must be a contiguous int32 or int64 [streams + 1] tensor")
-    return cu_seqlens.shape[0] - 1
+def _cu(what, cu_seqlens):
+    """(streams, dtype code) of cu_seqlens."""
+    shape, code = cu_seqlens.shape, _CODES.get(cu_seqlens.dtype)
+    if len(shape) != 1 or code not in (_mm.MM_INT32, _mm.MM_INT64) or shape[0] < 1 or not cu_seqlens.is_contiguous():
+        raise ValueError(f"{what}: cu_seqlens must be a contiguous int32 or int64 [streams + 1] tensor (got "
+                         f"{cu_seqlens.dtype} {list(shape)})")
+    return shape[0] - 1, code
 
 
-def _batch(page_table, cu_seqlens, kv_lens, tokens, what):
-    B = _cu(cu_seqlens, what)
+def _batch(what, page_table, cu_seqlens, kv_lens, tokens):
+    """(mm_batch, streams, pages of a row of the table)."""
+    B, code = _cu(what, cu_seqlens)
+    it = cu_seqlens.dtype
+    if kv_lens.dtype is not it or page_table.dtype is not it:
+        raise ValueError(f"{what}: cu_seqlens, kv_lens and page_table must have one dtype (got {it}, {kv_lens.dtype}, "
+                         f"{page_table.dtype})")
     if kv_lens.shape != (B,) or not kv_lens.is_contiguous():
-        raise ValueError(f"{what}: kv_lens must be a contiguous [{B}] tensor (got {tuple(kv_lens.shape)})")
-    if page_table.dim() != 2 or page_table.shape[0] != B or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
-        raise ValueError(f"{what}: page_table must be [{B}, pages] with contiguous rows (got {tuple(page_table.shape)})")
-    if not cu_seqlens.dtype == kv_lens.dtype == page_table.dtype:
-        raise ValueError(f"{what}: cu_seqlens, kv_lens and page_table must have one dtype (got {cu_seqlens.dtype}, "
-                         f"{kv_lens.dtype}, {page_table.dtype})")
-    return _mm.Batch(cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                     page_table.shape[1], B, tokens, _mm.dtype_code(cu_seqlens))
+        raise ValueError(f"{what}: kv_lens must be a contiguous [{B}] tensor (got {list(kv_lens.shape)})")
+    shape, s = page_table.shape, page_table.stride()
+    if len(shape) != 2 or shape[0] != B or (s[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: page_table must be [{B}, pages] with contiguous rows (got {list(shape)}, strides {s})")
+    pages = shape[1]
+    return (_BATCH.pack(cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), s[0], pages, B,
+                        tokens, code), B, pages)
+
+
+def _call(what, dev, fn, *args):
+    """fn(*args, stream) on device dev's current stream, with dev current."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _mm.check(rc, what)
 
 
 def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv_freq=None, *, rot_offset=0,
@@ -86,46 +133,51 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv
     exist (kv_lens outside the table, a page id outside the pool) stores nothing. Streams that share pages must not
     append to the same rows."""
     what = "paged_append"
-    _mm.require_gpu(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv_freq, q_out, k_out)
-    g = _pages(k_pages, v_pages, what)
-    dt = k_pages.dtype
-    qr = _rows(q, "q", what, None, g.dqk, dt)
-    N, nh = q.shape[0], q.shape[1]
-    kr, vr = _rows(k, "k", what, g.nkv, g.dqk, dt), _rows(v, "v", what, g.nkv, g.dv, dt)
-    if k.shape[0] != N or v.shape[0] != N:
-        raise ValueError(f"{what}: q, k and v must hold the same tokens (got {N}, {k.shape[0]}, {v.shape[0]})")
-    b = _batch(page_table, cu_seqlens, kv_lens, N, what)
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous()):
-        raise ValueError(f"{what}: inv_freq must be a contiguous fp32 [pairs] tensor")
+    dev = _device(what, q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv_freq, q_out, k_out)
+    pool, nkv, _, dqk, dv, dt = _pool(what, k_pages, v_pages)
+    N, nh, *qr = _queries(what, q, dqk, dt)
+    kr, vr = _rows(what, "k", k, (N, nkv, dqk), dt), _rows(what, "v", v, (N, nkv, dv), dt)
+    batch, _, _ = _batch(what, page_table, cu_seqlens, kv_lens, N)
+    if not 0 <= rot_offset <= dqk:
+        raise ValueError(f"{what}: rot_offset={rot_offset} lies outside a head of {dqk}")
+    inv, pairs = None, 0
+    if inv_freq is not None:
+        if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError(f"{what}: inv_freq must be a contiguous fp32 [pairs] tensor (got {inv_freq.dtype} "
+                             f"{list(inv_freq.shape)})")
+        inv, pairs = inv_freq.data_ptr(), inv_freq.shape[0]
     if q_out is None:
-        q_out = torch.empty(N, nh, g.dqk, device=q.device, dtype=dt)
-    elif q_out.shape[0] != N:
-        raise ValueError(f"{what}: q_out must hold {N} tokens (got {q_out.shape[0]})")
-    qo = _rows(q_out, "q_out", what, nh, g.dqk, dt)
-    if k_out is not None and k_out.shape[0] != N:
-        raise ValueError(f"{what}: k_out must hold {N} tokens (got {k_out.shape[0]})")
-    ko = (None, 0, 0) if k_out is None else _rows(k_out, "k_out", what, g.nkv, g.dqk, dt)
-    with _mm.on_device(q):
-        _mm.check(_mm.load().mm_paged_append(*qr, *kr, *vr, nh, g, b, _mm.ptr(inv_freq),
-                                             inv_freq.shape[0] if inv_freq is not None else 0, int(rot_offset),
-                                             1 if interleaved else 0, *qo, *ko, _mm.stream_of(q)), what)
+        q_out = torch.empty(N, nh, dqk, device=q.device, dtype=dt)
+    qo = _rows(what, "q_out", q_out, (N, nh, dqk), dt)
+    ko = (None, 0, 0) if k_out is None else _rows(what, "k_out", k_out, (N, nkv, dqk), dt)
+    _call(what, dev, _mm.load().mm_paged_append, *qr, *kr, *vr, nh, pool, batch, inv, pairs, int(rot_offset),
+          1 if interleaved else 0, *qo, *ko)
     return q_out
 
 
-def _workspace(n, device, what, workspace):
-    """The workspace of n bytes: the caller's, or a new one; None where none is needed."""
+def _workspace(n, like, workspace):
+    """The workspace of n bytes: the caller's, or a new one where one is needed. A new one lives until its call's kernels
+    are enqueued; what the allocator then hands out of it comes behind them on the stream."""
+    if workspace is None and n > 0:  # else none is needed, or the call itself refuses the sizes
+        workspace = torch.empty(n, dtype=torch.uint8, device=like.device)
+    return workspace
+
+
+def _bytes(workspace):
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def _new_workspace(what, n, device):
     if n < 0:
         raise ValueError(f"{what}: {_mm.last_error()}")
-    if workspace is None:
-        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    return workspace
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def paged_attn_workspace(tokens, streams, max_keys, nh, nkv, dqk, dv, device="cuda"):
     """The workspace paged_attn needs for a batch of up to `tokens` tokens in `streams` streams behind a table of max_keys
     = pages * page positions (no initialisation); calls that share it must not overlap in time."""
     n = _mm.load().mm_paged_attn_workspace(tokens, streams, max_keys, nh, nkv, dqk, dv)
-    return _workspace(max(n, 16) if n >= 0 else n, device, "paged_attn_workspace", None)
+    return _new_workspace("paged_attn_workspace", n, device)
 
 
 def paged_attn(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, scale=None, out=None, workspace=None):
@@ -137,23 +189,16 @@ def paged_attn(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, scale=None,
     gives NaN. Rows past a token's position never reach it, whatever they hold. out must not overlap q or the pool.
     workspace: from paged_attn_workspace (allocated when None)."""
     what = "paged_attn"
-    _mm.require_gpu(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, out, workspace)
-    g = _pages(k_pages, v_pages, what)
-    dt = k_pages.dtype
-    qr = _rows(q, "q", what, None, g.dqk, dt)
-    N, nh = q.shape[0], q.shape[1]
-    b = _batch(page_table, cu_seqlens, kv_lens, N, what)
+    dev = _device(what, q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, out, workspace)
+    pool, nkv, page, dqk, dv, dt = _pool(what, k_pages, v_pages)
+    N, nh, *qr = _queries(what, q, dqk, dt)
+    batch, B, pages = _batch(what, page_table, cu_seqlens, kv_lens, N)
     if out is None:
-        out = torch.empty(N, nh, g.dv, device=q.device, dtype=dt)
-    elif out.shape[0] != N:
-        raise ValueError(f"{what}: out must hold {N} tokens (got {out.shape[0]})")
-    o = _rows(out, "out", what, nh, g.dv, dt)
+        out = torch.empty(N, nh, dv, device=q.device, dtype=dt)
+    o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
-    with _mm.on_device(q):
-        ws = _workspace(lib.mm_paged_attn_workspace(N, b.seqs, b.max_pages * g.page, nh, g.nkv, g.dqk, g.dv), q.device, what,
-                        workspace)
-        _mm.check(lib.mm_paged_attn(*qr, nh, g, b, float(scale) if scale is not None else g.dqk ** -0.5, *o, _mm.ptr(ws),
-                                    ws.numel() * ws.element_size() if ws is not None else 0, _mm.stream_of(q)), what)
+    ws = _workspace(lib.mm_paged_attn_workspace(N, B, pages * page, nh, nkv, dqk, dv), q, workspace)
+    _call(what, dev, lib.mm_paged_attn, *qr, nh, pool, batch, dqk ** -0.5 if scale is None else float(scale), *o, *_bytes(ws))
     return out
 
 
@@ -161,7 +206,7 @@ def prompt_attn_workspace(tokens, prompts, nh, nkv, dqk, dv, device="cuda"):
     """The workspace prompt_attn needs for up to `tokens` tokens in `prompts` prompts (no initialisation); calls that
     share it must not overlap in time."""
     n = _mm.load().mm_prompt_attn_workspace(tokens, prompts, nh, nkv, dqk, dv)
-    return _workspace(max(n, 16) if n >= 0 else n, device, "prompt_attn_workspace", None)
+    return _new_workspace("prompt_attn_workspace", n, device)
 
 
 def prompt_attn(q, k, v, cu_seqlens, scale=None, out=None, workspace=None):
@@ -171,27 +216,22 @@ def prompt_attn(q, k, v, cu_seqlens, scale=None, out=None, workspace=None):
     [tokens, nh, dv] (scale defaults to dqk ** -0.5). Rounding, rows behind the last prompt and workspace (from
     prompt_attn_workspace) as for paged_attn. out must not overlap q, k or v."""
     what = "prompt_attn"
-    _mm.require_gpu(q, k, v, cu_seqlens, out, workspace)
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{what}: q must be bf16 or fp16 (got {q.dtype})")
+    dev = _device(what, q, k, v, cu_seqlens, out, workspace)
     dt = q.dtype
-    qr = _rows(q, "q", what)
-    N, nh, dqk = q.shape
-    kr, vr = _rows(k, "k", what, None, dqk, dt), _rows(v, "v", what, k.shape[1], None, dt)
-    nkv, dv = v.shape[1:]
-    if k.shape[0] != N or v.shape[0] != N:
-        raise ValueError(f"{what}: q, k and v must hold the same tokens (got {N}, {k.shape[0]}, {v.shape[0]})")
-    B = _cu(cu_seqlens, what)
+    if dt not in _HALF:
+        raise ValueError(f"{what}: q must be bf16 or fp16 (got {dt})")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"{what}: q, k and v must be [tokens, heads, d] (got {list(q.shape)}, {list(k.shape)}, "
+                         f"{list(v.shape)})")
+    nkv, dqk, dv = k.shape[1], k.shape[2], v.shape[2]
+    N, nh, *qr = _queries(what, q, dqk, dt)
+    kr, vr = _rows(what, "k", k, (N, nkv, dqk), dt), _rows(what, "v", v, (N, nkv, dv), dt)
+    B, code = _cu(what, cu_seqlens)
     if out is None:
         out = torch.empty(N, nh, dv, device=q.device, dtype=dt)
-    elif out.shape[0] != N:
-        raise ValueError(f"{what}: out must hold {N} tokens (got {out.shape[0]})")
-    o = _rows(out, "out", what, nh, dv, dt)
+    o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
-    with _mm.on_device(q):
-        ws = _workspace(lib.mm_prompt_attn_workspace(N, B, nh, nkv, dqk, dv), q.device, what, workspace)
-        _mm.check(lib.mm_prompt_attn(*qr, *kr, *vr, _mm.dtype_code(q), nh, nkv, dqk, dv, _mm.ptr(cu_seqlens),
-                                     _mm.dtype_code(cu_seqlens), B, N, float(scale) if scale is not None else dqk ** -0.5,
-                                     *o, _mm.ptr(ws), ws.numel() * ws.element_size() if ws is not None else 0,
-                                     _mm.stream_of(q)), what)
+    ws = _workspace(lib.mm_prompt_attn_workspace(N, B, nh, nkv, dqk, dv), q, workspace)
+    _call(what, dev, lib.mm_prompt_attn, *qr, *kr, *vr, _CODES[dt], nh, nkv, dqk, dv, cu_seqlens.data_ptr(), code, B, N,
+          dqk ** -0.5 if scale is None else float(scale), *o, *_bytes(ws))
     return out

@@ -172,6 +172,7 @@ def test_wrappers_take_gpu_tensors_only():
 def any_device(monkeypatch):
     """The wrappers' own checks on CPU tensors: none of the refused calls reaches the library."""
     monkeypatch.setattr(mm, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(PK, "_call", lambda *a: pytest.fail("the call was not refused"))
 
 
 def _args(N=3, B=2, nh=4, nkv=2, d=16, dv=8, dt=BF, idx=torch.int32):
@@ -185,8 +186,10 @@ def _args(N=3, B=2, nh=4, nkv=2, d=16, dv=8, dt=BF, idx=torch.int32):
     ("q must be", dict(q=torch.zeros(3, 4, 24, dtype=BF))), ("q must be", dict(q=torch.zeros(3, 64, dtype=BF))),
     ("q must be", dict(q=torch.zeros(3, 4, 16))), ("contiguous last dim", dict(q=torch.zeros(3, 16, 4, dtype=BF).mT)),
     ("k must be", dict(k=torch.zeros(3, 3, 16, dtype=BF))), ("v must be", dict(v=torch.zeros(3, 2, 16, dtype=BF))),
-    ("same tokens", dict(k=torch.zeros(4, 2, 16, dtype=BF))),
+    ("k must be", dict(k=torch.zeros(4, 2, 16, dtype=BF))), ("rot_offset=-8", dict(rot_offset=-8)),
+    ("rot_offset", dict(rot_offset=1 << 32)),
     ("k_pages and v_pages must be", dict(k_pages=torch.zeros(5, 2, 8, 16, dtype=BF))),
+    ("k_pages and v_pages must both", dict(k_pages=torch.zeros(5, 2, 16, dtype=BF))),
     ("both be bf16 or fp16", dict(k_pages=torch.zeros(5, 2, 4, 16))),
     ("kv_lens must be", dict(kv_lens=torch.zeros(3, dtype=torch.int32))),
     ("one dtype", dict(kv_lens=torch.zeros(2, dtype=torch.int64))), ("cu_seqlens", dict(cu_seqlens=torch.zeros(3))),
@@ -194,8 +197,8 @@ def _args(N=3, B=2, nh=4, nkv=2, d=16, dv=8, dt=BF, idx=torch.int32):
     ("page_table", dict(page_table=torch.zeros(3, 3, dtype=torch.int32))),
     ("page_table", dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t())),
     ("inv_freq", dict(inv_freq=torch.zeros(8, dtype=BF))), ("q_out", dict(q_out=torch.zeros(3, 4, 8, dtype=BF))),
-    ("q_out must hold 3", dict(q_out=torch.zeros(2, 4, 16, dtype=BF))),
-    ("k_out must hold 3", dict(k_out=torch.zeros(2, 2, 16, dtype=BF)))])
+    ("q_out must be", dict(q_out=torch.zeros(2, 4, 16, dtype=BF))),
+    ("k_out must be", dict(k_out=torch.zeros(2, 2, 16, dtype=BF)))])
 def test_append_wrapper_refuses(any_device, what, change):
     with pytest.raises(ValueError, match=what):
         PK.paged_append(**{**_args(), **change})
@@ -204,7 +207,7 @@ def test_append_wrapper_refuses(any_device, what, change):
 @pytest.mark.parametrize("what,change", [
     ("q must be", dict(q=torch.zeros(3, 4, 24, dtype=BF))), ("q must be", dict(q=torch.zeros(3, 4, 16, dtype=torch.float16))),
     ("k_pages and v_pages must be", dict(v_pages=torch.zeros(4, 2, 4, 8, dtype=BF))),
-    ("out must hold 3", dict(out=torch.zeros(2, 4, 8, dtype=BF))), ("out must be", dict(out=torch.zeros(3, 4, 16, dtype=BF))),
+    ("out must be", dict(out=torch.zeros(2, 4, 8, dtype=BF))), ("out must be", dict(out=torch.zeros(3, 4, 16, dtype=BF))),
     ("one dtype", dict(page_table=torch.zeros(2, 3, dtype=torch.int64)))])
 def test_attn_wrapper_refuses(any_device, what, change):
     a = {k: v for k, v in _args().items() if k not in "kv"}
@@ -213,8 +216,9 @@ def test_attn_wrapper_refuses(any_device, what, change):
 
 
 @pytest.mark.parametrize("what,change", [
-    ("bf16 or fp16", dict(q=torch.zeros(3, 4, 16))), ("k must be", dict(k=torch.zeros(3, 2, 8, dtype=BF))),
-    ("v must be", dict(v=torch.zeros(3, 1, 8, dtype=BF))), ("same tokens", dict(v=torch.zeros(2, 2, 8, dtype=BF))),
+    ("bf16 or fp16", dict(q=torch.zeros(3, 4, 16))), ("q must be", dict(k=torch.zeros(3, 2, 8, dtype=BF))),
+    ("k must be", dict(k=torch.zeros(4, 2, 16, dtype=BF))),
+    ("v must be", dict(v=torch.zeros(3, 1, 8, dtype=BF))), ("v must be", dict(v=torch.zeros(2, 2, 8, dtype=BF))), ("q, k and v must be", dict(v=torch.zeros(3, 16, dtype=BF))),
     ("cu_seqlens", dict(cu_seqlens=torch.zeros(2, 2, dtype=torch.int32))),
     ("out must be", dict(out=torch.zeros(3, 4, 8)))])
 def test_prompt_wrapper_refuses(any_device, what, change):
