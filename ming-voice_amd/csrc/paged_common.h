@@ -282,11 +282,6 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
   return (w & lo) == lo || (w & hi) == hi;
 }
 
-template <class T>
-__device__ __forceinline__ float value_of(uint32_t bits) {  // of the low half
-  return T::kBf16 ? __uint_as_float(bits << 16) : f16_to_f32(static_cast<uint16_t>(bits));
-}
-
 // The page number read for a key, as it came (both halves of a 64-bit entry; the same word twice of a 32-bit one), so
 // that nothing waits for it before it is used.
 struct PageId {
@@ -305,6 +300,94 @@ __device__ __forceinline__ bool page_ok(const AttnArgs& a, PageId id) {
 
 // What a row that does not exist reads.
 static __device__ const uint4 kZeroRow[32] = {};
+
+// One row of a block over the keys k_begin .. k_end - 1 of its stream, key by key, by one wave: what the matrix units cannot
+// do where a key that the row must not see holds an infinity or a NaN in its values (0 * inf). Few tiles can hold such a
+// key at all (those that some rows of the block see and others do not), the kernels look into these, and rows of a block
+// that met one are computed anew here. Lane l ends with the sums of dims l + 64 e.
+struct RowSums {
+  float acc[4], m, l;  // m in units of log2 of the weight
+};
+
+template <class T>
+__device__ __forceinline__ RowSums row_by_keys(const AttnArgs& a, const Work& w, int kvh, int row, int k_begin, int k_end) {
+  const int lane = lane_id(), i = static_cast<int>(div_by(row, a.group));
+  const uint16_t* q = a.q.at(w.s.first + i, kvh * static_cast<int>(a.group.d) + row - i * static_cast<int>(a.group.d));
+  const int end = min(k_end, w.s.kv - w.s.n + i + 1);
+  const float sc = (a.negative ? -a.scale : a.scale) * 1.4426950408889634f;
+  RowSums r{{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f};
+#pragma unroll 1
+  for (int k0 = k_begin; k0 < end; k0 += kWave) {
+    const int key = min(k0 + lane, end - 1);
+    bool ok = k0 + lane < end;
+    const uint16_t *kr, *vr;
+    if (a.batch.table) {
+      const PageId id = page_id(a, w.b, key);
+      ok = ok && page_ok(a, id);
+      const int at = key - static_cast<int>(div_by(key, a.page)) * static_cast<int>(a.page.d);
+      kr = a.kp.at(static_cast<int>(id.lo), kvh, at);
+      vr = a.vp.at(static_cast<int>(id.lo), kvh, at);
+    } else {
+      kr = a.k.at(w.s.first + key, kvh);
+      vr = a.v.at(w.s.first + key, kvh);
+    }
+    float s = 0.f;
+    if (ok) {
+#pragma unroll 1
+      for (int d = 0; d < a.dqk; d += 8) {
+        float x[8], y[8];
+        unpack8<T>(ld16(kr + d), x);
+        unpack8<T>(ld16(q + d), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
+    }
+    s = ok ? s * sc : -INFINITY;
+    const float mn = fmaxf(r.m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
+    const float p = ok ? exp2_fast(s - mu) : 0.f, alpha = exp2_fast(r.m - mu);
+    r.m = mn;
+    r.l = fmaf(r.l, alpha, wave_sum(p));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.acc[e] *= alpha;
+    const uint64_t all = __ballot(ok), v = reinterpret_cast<uint64_t>(vr);
+#pragma unroll 1
+    for (int j = 0; j < kWave; ++j) {
+      if (!((all >> j) & 1)) continue;
+      const float pj = __shfl(p, j, kWave);
+      const auto* vj = reinterpret_cast<const uint16_t*>((static_cast<uint64_t>(__shfl(static_cast<uint32_t>(v >> 32), j, kWave)) << 32) |
+                                                         __shfl(static_cast<uint32_t>(v), j, kWave));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + kWave * e < a.dv) r.acc[e] = fmaf(pj, T::ld(vj, lane + kWave * e), r.acc[e]);
+    }
+  }
+  return r;
+}
+
+// The rows first, first + step, .. of a block's `rows` by row_by_keys, into the outputs or, where the block is cut, into
+// the piece's state.
+template <class T, int BR>
+__device__ __forceinline__ void rows_by_keys(const AttnArgs& a, const Work& w, int kvh, int rows, int first, int step, int k_begin,
+                                             int k_end, float* state) {
+  const int lane = lane_id(), G = static_cast<int>(a.group.d);
+#pragma unroll 1
+  for (int r = first; r < rows; r += step) {
+    const int row = w.blk * BR + r, i = static_cast<int>(div_by(row, a.group));
+    const RowSums s = row_by_keys<T>(a, w, kvh, row, k_begin, k_end);
+    uint16_t* out = a.out.at(w.s.first + i, kvh * G + row - i * G);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = lane + kWave * e;
+      if (d >= a.dv) break;
+      if (state) state[r * a.dv + d] = s.acc[e];
+      else T::st(out, d, s.m == -INFINITY ? 0.f : s.acc[e] / s.l);
+    }
+    if (state && lane == 0) {
+      state[BR * a.dv + r] = s.m;
+      state[BR * a.dv + BR + r] = s.l;
+    }
+  }
+}
 
 // What a call launches. Few rows to a block (16) or many (128); target: pieces of keys aimed at for the whole batch (0: no
 // cutting, no join); blocks: the most row blocks that these sizes can have.

@@ -19,7 +19,8 @@ struct Few {
   static constexpr int K_BYTES = kKeys * KC * 16, V_BYTES = kKeys * VC * 16;
   static constexpr int OROW = DVM + 4;
   static constexpr int ML = BR * OROW;                   // the wave's maxima and sums, after its outputs
-  static constexpr int O_BYTES = (ML + 2 * BR) * 4;
+  static constexpr int MET = ML + 2 * BR;                // and whether it met a value that is not finite
+  static constexpr int O_BYTES = (MET + 4) * 4;
   static constexpr int WAVE_BYTES = K_BYTES + V_BYTES > O_BYTES ? K_BYTES + V_BYTES : O_BYTES;
   static constexpr size_t LDS = static_cast<size_t>(NW) * WAVE_BYTES;
   static_assert(LDS <= 160 * 1024 && KI % 2 == 0 && NT % 4 == 0, "tile shape");
@@ -36,7 +37,7 @@ struct Few {
 // requested as soon as this one's are in registers, its values as soon as this one's are; the page numbers of the tile
 // after that are read one tile ahead, lane l for key l % 32, and handed to the loading lanes by ds_bpermute. Keys that no
 // row sees (past the piece, in a missing page) read a row of zeros. A value that some rows must not see could still be an
-// infinity or NaN (0 * inf): such tiles take their values key by key.
+// infinity or NaN (0 * inf): the waves look for it in the tiles that can hold one (row_by_keys).
 template <class T, int QF, int NW, int NKQ, int NT, bool PAGED>
 __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   using P = Few<QF, NW, NKQ, NT>;
@@ -152,6 +153,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
     for (int nt = 0; nt < NT; ++nt) o[f][nt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   const float sc = a.scale * 1.4426950408889634f;  // scores in units of log2: exp2 gives the weights
+  bool bad = false;
   if (wave < tiles) {
     PageId next{0, 0};
     if constexpr (PAGED) next = page_id(a, w.b, key_of(wave));
@@ -187,14 +189,13 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
         for (int f = 0; f < QF; ++f)
 #pragma unroll
           for (int u = 0; u < 2; ++u) s[f][u] = Mfma<T>::m16(kx[u][kk], qf[f][kk], s[f][u]);
-      const bool mixed = j0 + kKeys > lim_all;  // some row does not see some key that exists
-      uint32_t sees[QF];
+      const bool mixed = j0 + kKeys > lim_all;  // some row does not see some key: its value must be finite, or 0 * inf reaches the row
       uint4 pf[QF];
 #pragma unroll
       for (int f = 0; f < QF; ++f) {
         const int n = lim[f] - j0;
-        sees[f] = n >= kKeys ? mine : n <= 0 ? 0u : mine & ((1u << n) - 1u);
-        const uint32_t lo4 = sees[f] >> (4 * lq), hi4 = sees[f] >> (16 + 4 * lq);
+        const uint32_t sees = n >= kKeys ? mine : n <= 0 ? 0u : mine & ((1u << n) - 1u);
+        const uint32_t lo4 = sees >> (4 * lq), hi4 = sees >> (16 + 4 * lq);
         float sv[8];
         float tmax = -INFINITY;
 #pragma unroll
@@ -236,30 +237,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
         for (int b = 0; b < 4; ++b) {
           const uint4 vf = make_uint4(static_cast<uint32_t>(lo[b]), static_cast<uint32_t>(lo[b] >> 32),
                                       static_cast<uint32_t>(hi[b]), static_cast<uint32_t>(hi[b] >> 32));
-          // 0 * inf is NaN: where a row must not see a key whose value is not finite, the keys go one by one
-          if (mixed && __any(not_finite<T>(vf.x) || not_finite<T>(vf.y) || not_finite<T>(vf.z) || not_finite<T>(vf.w))) {
-#pragma unroll
-            for (int f = 0; f < QF; ++f) {
-              const uint32_t w0 = pf[f].x, w1 = pf[f].y, w2 = pf[f].z, w3 = pf[f].w;
-#pragma unroll 1
-              for (int key = 0; key < kKeys; ++key) {
-                const int e = key % 4 + 4 * (key / 16);
-                const uint32_t pw = e < 2 ? w0 : e < 4 ? w1 : e < 6 ? w2 : w3;
-                const uint32_t pk = static_cast<uint32_t>(
-                    __builtin_amdgcn_ds_bpermute(4 * (lr + 16 * (key % 16 / 4)), static_cast<int>(pw)));
-                const uint32_t see = (sees[f] >> key) & 1u ? ~0u : 0u;
-                const float p = value_of<T>((e & 1 ? pk >> 16 : pk) & see);
-                const int d = 16 * (n0 + b) + 4 * lq;
-                const uint2 x = *reinterpret_cast<const uint2*>(vt + key * P::VC * 16 + v_chunk_at<P::VC>(key, d / 8) * 16 + (d % 8) * 2);
-                floatx4& ob = o[f][n0 + b];
-                ob[0] = fmaf(p, value_of<T>(x.x & see), ob[0]);
-                ob[1] = fmaf(p, value_of<T>((x.x & see) >> 16), ob[1]);
-                ob[2] = fmaf(p, value_of<T>(x.y & see), ob[2]);
-                ob[3] = fmaf(p, value_of<T>((x.y & see) >> 16), ob[3]);
-              }
-            }
-            continue;
-          }
+          if (mixed) bad = bad || not_finite<T>(vf.x) || not_finite<T>(vf.y) || not_finite<T>(vf.z) || not_finite<T>(vf.w);
 #pragma unroll
           for (int f = 0; f < QF; ++f) o[f][n0 + b] = Mfma<T>::m16(vf, pf[f], o[f][n0 + b]);
         }
@@ -283,8 +261,17 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
       so[P::ML + BR + 16 * f + lr] = l[f];
     }
   }
+  const bool mine_met = __any(bad);
+  if (lane == 0) so[P::MET] = mine_met ? 1.f : 0.f;
   __syncthreads();
   float* state = pieces > 1 ? state_at<BR>(a, w.slot + w.piece, kvh) : nullptr;
+  float met = 0.f;
+#pragma unroll
+  for (int x = 0; x < NW; ++x) met += reinterpret_cast<const float*>(s_few + x * P::WAVE_BYTES)[P::MET];
+  if (__builtin_amdgcn_readfirstlane(met != 0.f)) {
+    rows_by_keys<T, BR>(a, w, kvh, rows, wave, NW, k_begin, k_end, state);
+    return;
+  }
   for (int i = tid; i < rows * n4; i += NW * kWave) {
     const int r = i / n4, d = 4 * (i - r * n4);
     auto of = [&](int x) { return reinterpret_cast<const float*>(s_few + x * P::WAVE_BYTES); };

@@ -10,23 +10,22 @@ constexpr int kKeys = 64;   // keys per tile
 constexpr int kWaves = 4;
 constexpr int kRows = 32;   // rows per wave
 
-// The shape of many_kernel: head dims up to 16 NK (q, k) and 32 ND (v).
-template <int NK, int ND>
+// The shape of many_kernel: head dims up to 64 KS (q, k) and 64 VS (v). A tile lies in LDS as pieces of 64 keys by 64 dims,
+// 8 KB each: every load instruction then fills 8 rows of 128 bytes, whatever the head dims are.
+template <int KS, int VS>
 struct Many {
   static constexpr int BR = kWaves * kRows;
   static constexpr int GR = kKeys;
-  static constexpr int KC = 2 * NK, VC = 4 * ND;  // 16-byte chunks of a key, value row in LDS
-  static constexpr int KI = KC / kWaves, VI = VC / kWaves;  // loads per thread, key and value tile
-  static constexpr int K_BYTES = kKeys * KC * 16, V_BYTES = kKeys * VC * 16;
-  static_assert(2 * (K_BYTES + V_BYTES) <= 159 * 1024 && KC % kWaves == 0 && VC % kWaves == 0, "tile shape");
+  static constexpr int PIECE = kKeys * 128;  // bytes
+  static constexpr int K_BYTES = KS * PIECE, V_BYTES = VS * PIECE;
+  static_assert(2 * (K_BYTES + V_BYTES) <= 159 * 1024, "tile shape");
 };
 
-// The chunk of a value row held at LDS place c of the row: the 4 rows that 32 lanes of a transposing read take 64 bytes
-// of fall on distinct banks.
-template <int VC>
-__device__ __forceinline__ int v_chunk_of(int row, int c) {
-  return VC == 8 ? c ^ (4 * ((row >> 1) & 1)) : c ^ (4 * (row & 3));
-}
+// The chunk of a piece's row held at LDS place c of the row (involutions). Keys: the 16 rows that a fragment reads at one
+// chunk fall on the 16 distinct 16-byte columns of the banks; values: the 4 rows of which 32 lanes of a transposing read
+// take 64 bytes each fall on distinct quarters.
+__device__ __forceinline__ int k_swizzle(int row, int c) { return c ^ ((row >> 1) & 7); }
+__device__ __forceinline__ int v_swizzle(int row, int c) { return c ^ (4 * ((row >> 1) & 1)); }
 
 // 8 keys of a 32-dim tile of V^T as the 32x32x16 MFMA takes them: 4 rows from place p on and the 4 rows `hi` bytes on, each
 // read transposed (lane layout: lds_tr4x2). By the builtin: the waits are the compiler's.
@@ -44,13 +43,15 @@ __device__ __forceinline__ float half_max(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-template <class T, int NK, int ND, bool PAGED>
-__global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(AttnArgs a) {
-  using P = Many<NK, ND>;
-  constexpr int BR = P::BR;
+// Where a tile's rows come from, chosen on the host (rows_of_kind).
+enum Source { kPacked, kPaged, kAnywhere };
+
+template <class T, int KS, int VS, int SRC>
+__global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(AttnArgs a) {
+  using P = Many<KS, VS>;
+  constexpr int BR = P::BR, NK = 4 * KS, ND = 2 * VS;
   // two buffers, each an object of its own: reads of one then need not wait for the loads in flight into the other
   __shared__ __align__(1024) char s_k0[P::K_BYTES], s_v0[P::V_BYTES], s_k1[P::K_BYTES], s_v1[P::V_BYTES];
-  __shared__ int s_flag[2];  // a tile holds a value that is not finite
   const int tid = threadIdx.x, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lr = lane & 31, lh = lane >> 5, G = static_cast<int>(a.group.d);
@@ -73,55 +74,85 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
   const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;
   const int ctx = w.s.kv - w.s.n;
 
-  // load i of a wave fills LDS chunks 64 (4 i + wave) + lane of a tile: row krow[i], dims kdim[i] ..
-  int krow[P::KI], kdim[P::KI], vrow[P::VI], vdim[P::VI];
-#pragma unroll
-  for (int i = 0; i < P::KI; ++i) {
-    const int c = kWave * (kWaves * i + wave) + lane;
-    krow[i] = c / P::KC;
-    kdim[i] = 8 * k_chunk_at<P::KC>(krow[i], c % P::KC);
-  }
-#pragma unroll
-  for (int i = 0; i < P::VI; ++i) {
-    const int c = kWave * (kWaves * i + wave) + lane;
-    vrow[i] = c / P::VC;
-    vdim[i] = 8 * v_chunk_of<P::VC>(vrow[i], c % P::VC);
-  }
+  // A wave fills rows 8 wave .. + 7 and 32 + 8 wave .. + 7 of each piece, lane l row l / 8 of them at LDS place l % 8.
+  const int lrow = lane / 8, kdim = 8 * k_swizzle(8 * wave + lrow, lane % 8), vdim = 8 * v_swizzle(8 * wave + lrow, lane % 8);
+  uint64_t there = 0;  // the tile's keys that exist
+  // kPacked, kPaged: the 8 rows of a load lie side by side, in one page: a buffer resource from the first of them to the end
+  // of the last that exists; dims past the head's end lie past every resource
+  const uint32_t krs = static_cast<uint32_t>(SRC == kPacked ? a.k.ts : a.kp.rs) * 2u, vrs = static_cast<uint32_t>(SRC == kPacked ? a.v.ts : a.vp.rs) * 2u;
+  const uint32_t koff = lrow * krs + 2u * kdim, voff = lrow * vrs + 2u * vdim;
+  // kAnywhere: lane l finds key l's rows and hands them to the loading lanes
   const char* zeros = reinterpret_cast<const char*>(kZeroRow);
-  auto key_of = [&](int it) { return min(k_begin + it * kKeys + lane, k_end - 1); };
-  const char *kr, *vr;  // lane l: key l's rows of the tile being loaded
-  uint64_t there = 0;   // and which keys exist
-  auto find_rows = [&](int it, PageId id) {
-    const int key = k_begin + it * kKeys + lane, kc = min(key, k_end - 1);
-    bool ok = key < k_end;
-    if constexpr (PAGED) {
-      ok = ok && page_ok(a, id);
-      const int row = kc - static_cast<int>(div_by(kc, a.page)) * static_cast<int>(a.page.d);
-      kr = reinterpret_cast<const char*>(a.kp.at(static_cast<int>(id.lo), kvh, row));
-      vr = reinterpret_cast<const char*>(a.vp.at(static_cast<int>(id.lo), kvh, row));
-    } else {
-      kr = reinterpret_cast<const char*>(a.k.at(w.s.first + kc, kvh));
-      vr = reinterpret_cast<const char*>(a.v.at(w.s.first + kc, kvh));
-    }
-    if (!ok) kr = vr = zeros;
-    there = __ballot(ok);
-  };
+  const char *kr = zeros, *vr = zeros;
   auto row_of = [&](const char* p, int r) {
     const uint64_t v = reinterpret_cast<uint64_t>(p);
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * r, static_cast<int>(v)));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * r, static_cast<int>(v >> 32)));
     return reinterpret_cast<const char*>((static_cast<uint64_t>(hi) << 32) | lo);
   };
-  auto load_tile = [&](char* kt, char* vt) {
-#pragma unroll
-    for (int i = 0; i < P::KI; ++i) {
-      const char* p = row_of(kr, krow[i]) + 2 * kdim[i];
-      load_lds16(kdim[i] < a.dqk ? p : zeros, kt + wave * 1024 + i * kWaves * 1024);
+  // the page numbers of a tile: of key l (kAnywhere), of keys 8 (l % 8) .. + 7 (kPaged)
+  auto ids_of = [&](int it) {
+    const int key = k_begin + it * kKeys + (SRC == kAnywhere ? lane : 8 * (lane % 8));
+    if (SRC == kPacked || (SRC == kAnywhere && !a.batch.table)) return PageId{0, 0};
+    return page_id(a, w.b, min(key, k_end - 1));
+  };
+  auto load_tile = [&](int it, PageId id, char* kt, char* vt) {
+    const int j0 = k_begin + it * kKeys, left = k_end - j0;  // keys of the tile and behind
+    if constexpr (SRC == kAnywhere) {
+      const int key = min(j0 + lane, k_end - 1);
+      bool ok = lane < left;
+      if (a.batch.table) {
+        ok = ok && page_ok(a, id);
+        const int row = key - static_cast<int>(div_by(key, a.page)) * static_cast<int>(a.page.d);
+        kr = reinterpret_cast<const char*>(a.kp.at(static_cast<int>(id.lo), kvh, row));
+        vr = reinterpret_cast<const char*>(a.vp.at(static_cast<int>(id.lo), kvh, row));
+      } else {
+        kr = reinterpret_cast<const char*>(a.k.at(w.s.first + key, kvh));
+        vr = reinterpret_cast<const char*>(a.v.at(w.s.first + key, kvh));
+      }
+      if (!ok) kr = vr = zeros;
+      there = __ballot(ok);
+    } else {
+      there = left >= kKeys ? ~0ull : (1ull << left) - 1;
+      if constexpr (SRC == kPaged) {
+        uint32_t bad = static_cast<uint32_t>(__ballot(!page_ok(a, id))) & 0xffu;  // by groups of 8 keys
+        while (bad) {
+          const int g = __builtin_ctz(bad);
+          bad &= bad - 1;
+          there &= ~(0xffull << (8 * g));
+        }
+      }
     }
 #pragma unroll
-    for (int i = 0; i < P::VI; ++i) {
-      const char* p = row_of(vr, vrow[i]) + 2 * vdim[i];
-      load_lds16(vdim[i] < a.dv ? p : zeros, vt + wave * 1024 + i * kWaves * 1024);
+    for (int i = 0; i < 2; ++i) {
+      const int r = 32 * i + 8 * wave;  // the load's first row
+      char* kd = kt + r * 128;
+      char* vd = vt + r * 128;
+      if constexpr (SRC == kAnywhere) {
+        const char *kp = row_of(kr, r + lrow) + 2 * kdim, *vp = row_of(vr, r + lrow) + 2 * vdim;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) load_lds16(kdim + 64 * s < a.dqk ? kp + 128 * s : zeros, kd + s * P::PIECE);
+#pragma unroll
+        for (int s = 0; s < VS; ++s) load_lds16(vdim + 64 * s < a.dv ? vp + 128 * s : zeros, vd + s * P::PIECE);
+      } else {
+        const int n = min(8, static_cast<int>(__popcll(there & (0xffull << r))));  // its rows that exist, the first ones
+        const uint16_t *kb, *vb;
+        if constexpr (SRC == kPaged) {
+          const int page = n ? __builtin_amdgcn_readlane(static_cast<int>(id.lo), 4 * i + wave) : 0;
+          const int row = (j0 + r) - static_cast<int>(div_by(j0 + r, a.page)) * static_cast<int>(a.page.d);
+          kb = a.kp.at(page, kvh, row);
+          vb = a.vp.at(page, kvh, row);
+        } else {
+          kb = a.k.at(w.s.first + j0 + r, kvh);
+          vb = a.v.at(w.s.first + j0 + r, kvh);
+        }
+        const rsrc_t kres = make_rsrc(kb, n ? (n - 1) * static_cast<int64_t>(krs) + 2 * a.dqk : 0);
+        const rsrc_t vres = make_rsrc(vb, n ? (n - 1) * static_cast<int64_t>(vrs) + 2 * a.dv : 0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) buf_lds16(kres, kdim + 64 * s < a.dqk ? koff + 128u * s : kPast, kd + s * P::PIECE);
+#pragma unroll
+        for (int s = 0; s < VS; ++s) buf_lds16(vres, vdim + 64 * s < a.dv ? voff + 128u * s : kPast, vd + s * P::PIECE);
+      }
     }
   };
 
@@ -146,10 +177,11 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
       qf[ks] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
     }
   }
-  // this lane's places in a tile: key row 32 u + lr, chunk 2 ks + lh; value rows 16 st + 4 lh + (lane % 16) / 4 (+ 8), dims
-  // 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4) .. + 3
+  // this lane's places in a piece: key row 32 u + lr, chunk 2 (ks % 4) + lh; value rows 16 st + 4 lh + (lane % 16) / 4
+  // (+ 8), dims 32 (dt % 2) + 16 ((lane / 16) % 2) + 4 (lane % 4) .. + 3
+  const int kplace = lr * 128 + k_swizzle(lr, lh) * 16;
   const int vfr = 4 * lh + (lane & 15) / 4;
-  const int vplace = vfr * P::VC * 16 + v_chunk_of<P::VC>(vfr, 2 * ((lane >> 4) & 1) + (lane & 3) / 2) * 16 + (lane & 1) * 8;
+  const int vplace = vfr * 128 + v_swizzle(vfr, 2 * ((lane >> 4) & 1) + (lane & 3) / 2) * 16 + (lane & 1) * 8;
   floatx16 o[ND];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -158,29 +190,26 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   const float sc = a.scale * 1.4426950408889634f;
 
-  if (tid < 2) s_flag[tid] = 0;
+  bool bad = false;
   PageId next{0, 0};
-  auto tile = [&](int it, char* kt, char* vt, char* kt_next, char* vt_next, int* flag, int* flag_next) {
+  auto tile = [&](int it, char* kt, char* vt, char* kt_next, char* vt_next) {
     const int j0 = k_begin + it * kKeys;
     const uint64_t mine = there;
     wait_vmcnt<0>();  // this wave's part of the tile
     __syncthreads();  // every wave's part; and the other buffer has been read
     if (it + 1 < tiles) {
-      find_rows(it + 1, next);
-      if constexpr (PAGED) next = page_id(a, w.b, key_of(it + 2));
-      load_tile(kt_next, vt_next);
+      const PageId id = next;
+      next = ids_of(it + 2);
+      load_tile(it + 1, id, kt_next, vt_next);
     }
-    const bool mixed = j0 + kKeys > lim_block;  // some row does not see some key: 0 * inf must not reach it
-    if (mixed) {
-      if (tid == 0) *flag_next = 0;
-      bool bad = false;
+    if (j0 + kKeys > lim_block) {  // some row does not see some key: its value must be finite, or 0 * inf reaches the row
 #pragma unroll
-      for (int i = 0; i < P::VI; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(vt + wave * 1024 + i * kWaves * 1024 + lane * 16);
-        bad = bad || not_finite<T>(x.x) || not_finite<T>(x.y) || not_finite<T>(x.z) || not_finite<T>(x.w);
-      }
-      if (bad) *flag = 1;
-      __syncthreads();
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 0; s < VS; ++s) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vt + s * P::PIECE + (32 * i + 8 * wave) * 128 + lane * 16);
+          bad = bad || not_finite<T>(x.x) || not_finite<T>(x.y) || not_finite<T>(x.z) || not_finite<T>(x.w);
+        }
     }
     if (j0 < lim_max) {
       floatx16 s[2];
@@ -192,7 +221,7 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
       for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + (32 * u + lr) * P::KC * 16 + k_chunk_at<P::KC>(lr, 2 * ks + lh) * 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(kt + (ks / 4) * P::PIECE + u * 4096 + (kplace ^ (32 * (ks % 4))));
           s[u] = Mfma<T>::m32(x, qf[ks], s[u]);
         }
       uint64_t sees = ~0ull;
@@ -232,54 +261,37 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
         }
         pf[st] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
       }
-      if (mixed && __builtin_amdgcn_readfirstlane(*flag) != 0) {
-        // key by key; lane: row lr, dims 32 dt + 8 (i / 4) + 4 lh + i % 4
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const uint32_t w0 = pf[st].x, w1 = pf[st].y, w2 = pf[st].z, w3 = pf[st].w;
-#pragma unroll 1
-          for (int k = 0; k < 16; ++k) {
-            const int e = k % 4 + 4 * (k / 8), key = 16 * st + k;
-            const uint32_t pw = e < 2 ? w0 : e < 4 ? w1 : e < 6 ? w2 : w3;
-            const uint32_t pk = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * (lr + 32 * (k % 8 / 4)), static_cast<int>(pw)));
-            const uint32_t see = (sees >> key) & 1u ? ~0u : 0u;
-            const float p = value_of<T>((e & 1 ? pk >> 16 : pk) & see);
+      for (int st = 0; st < 4; ++st)
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const uint2 x = *reinterpret_cast<const uint2*>(vt + key * P::VC * 16 + v_chunk_of<P::VC>(key, 4 * dt + i / 4) * 16 + 8 * lh);
-                o[dt][i] = fmaf(p, value_of<T>(x.x & see), o[dt][i]);
-                o[dt][i + 1] = fmaf(p, value_of<T>((x.x & see) >> 16), o[dt][i + 1]);
-                o[dt][i + 2] = fmaf(p, value_of<T>(x.y & see), o[dt][i + 2]);
-                o[dt][i + 3] = fmaf(p, value_of<T>((x.y & see) >> 16), o[dt][i + 3]);
-              }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt)
-            o[dt] = Mfma<T>::m32(v_frag(vt + (vplace ^ (64 * dt)) + 16 * st * P::VC * 16, 8 * P::VC * 16), pf[st], o[dt]);
-      }
+        for (int dt = 0; dt < ND; ++dt)
+          o[dt] = Mfma<T>::m32(v_frag(vt + (dt / 2) * P::PIECE + (vplace ^ (64 * (dt % 2))) + 16 * st * 128, 8 * 128), pf[st], o[dt]);
     }
   };
   if (tiles > 0) {
-    if constexpr (PAGED) next = page_id(a, w.b, key_of(0));
-    find_rows(0, next);
-    if constexpr (PAGED) next = page_id(a, w.b, key_of(1));
-    load_tile(s_k0, s_v0);
+    const PageId id = ids_of(0);
+    next = ids_of(1);
+    load_tile(0, id, s_k0, s_v0);
   }
   for (int it = 0; it < tiles; it += 2) {
-    tile(it, s_k0, s_v0, s_k1, s_v1, s_flag, s_flag + 1);
-    if (it + 1 < tiles) tile(it + 1, s_k1, s_v1, s_k0, s_v0, s_flag + 1, s_flag);
+    tile(it, s_k0, s_v0, s_k1, s_v1);
+    if (it + 1 < tiles) tile(it + 1, s_k1, s_v1, s_k0, s_v0);
+  }
+  float* state = pieces > 1 ? state_at<BR>(a, w.slot + w.piece, kvh) : nullptr;
+  // whether any wave met such a value: in words of the key buffer, which is no longer needed
+  __syncthreads();
+  int* met = reinterpret_cast<int*>(s_k0);
+  const bool mine_met = __any(bad);
+  if (lane == 0) met[wave] = mine_met;
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(met[0] | met[1] | met[2] | met[3])) {
+    rows_by_keys<T, BR>(a, w, kvh, rows, wave, kWaves, k_begin, k_end, state);
+    return;
   }
   if (lr >= wrows) return;
   l += __shfl_xor(l, 32, kWave);
   const int r = kRows * wave + lr;  // of the workgroup
-  if (pieces > 1) {
-    float* state = state_at<BR>(a, w.slot + w.piece, kvh);
+  if (state) {
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -305,26 +317,35 @@ __global__ __launch_bounds__(kWaves * kWave, NK <= 12 ? 2 : 1) void many_kernel(
     }
 }
 
-template <class T, int NK, int ND, bool PAGED>
+template <class T, int KS, int VS, int SRC>
 int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL((many_kernel<T, NK, ND, PAGED>), dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)),
+  hipLaunchKernelGGL((many_kernel<T, KS, VS, SRC>), dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)),
                      dim3(kWaves * kWave), 0, st, a);
   return mm::check_launch(what);
 }
 
-template <class T, bool PAGED>
-int launch_type(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  if (a.dqk <= 64 && a.dv <= 64) return launch_shape<T, 4, 2, PAGED>(a, p, st, what);
-  if (a.dqk <= 128 && a.dv <= 128) return launch_shape<T, 8, 4, PAGED>(a, p, st, what);
-  if (a.dqk <= 192 && a.dv <= 128) return launch_shape<T, 12, 4, PAGED>(a, p, st, what);
-  return launch_shape<T, 16, 8, PAGED>(a, p, st, what);
+template <class T, int SRC>
+int launch_source(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
+  if (a.dqk <= 64 && a.dv <= 64) return launch_shape<T, 1, 1, SRC>(a, p, st, what);
+  if (a.dqk <= 128 && a.dv <= 128) return launch_shape<T, 2, 2, SRC>(a, p, st, what);
+  if (a.dqk <= 192 && a.dv <= 128) return launch_shape<T, 3, 2, SRC>(a, p, st, what);
+  return launch_shape<T, 4, 4, SRC>(a, p, st, what);
+}
+
+// Packed rows, and pages of a multiple of 8 rows, are read 8 rows to an instruction through a resource that ends with them
+// (a resource reaches 2^31 bytes); other pages, and rows further apart, row by row from wherever they lie.
+template <class T>
+int launch_type(const AttnArgs& a, const AttnPlan& p, bool paged, hipStream_t st, const char* what) {
+  const int64_t far = 1 << 26;  // elements between rows: 8 of them stay below 2^31 bytes
+  const bool near = paged ? a.page.d % 8 == 0 && a.kp.rs < far && a.vp.rs < far : a.k.ts < far && a.v.ts < far;
+  if (!near) return launch_source<T, kAnywhere>(a, p, st, what);
+  return paged ? launch_source<T, kPaged>(a, p, st, what) : launch_source<T, kPacked>(a, p, st, what);
 }
 
 }  // namespace
 
 int launch_many(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {
-  int rc = dtype == MM_BF16 ? (paged ? launch_type<BF16, true>(a, p, st, what) : launch_type<BF16, false>(a, p, st, what))
-                            : (paged ? launch_type<FP16, true>(a, p, st, what) : launch_type<FP16, false>(a, p, st, what));
+  int rc = dtype == MM_BF16 ? launch_type<BF16>(a, p, paged, st, what) : launch_type<FP16>(a, p, paged, st, what);
   if (rc || p.target == 0) return rc;
   return launch_join_many(a, p, dtype, st, what);
 }
