@@ -47,22 +47,35 @@ __device__ __forceinline__ int64_t idx_at(const void* p, int i64, int64_t i) {
   return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
 }
 
+// An index as it came: both halves of a 64-bit entry, the same word twice of a 32-bit one. Nothing waits for it, or
+// branches on its type, before it is used.
+struct Index {
+  uint32_t lo, hi;
+};
+
+__device__ __forceinline__ Index index_at(const void* p, int i64, int64_t i) {
+  const uint32_t* w = static_cast<const uint32_t*>(p) + (i64 ? 2 * i : i);
+  return Index{w[0], w[i64 ? 1 : 0]};
+}
+
+__device__ __forceinline__ int64_t value_of(Index x, int i64) {
+  const int hi = static_cast<int>(i64 ? x.hi : static_cast<uint32_t>(static_cast<int>(x.lo) >> 31));
+  return static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | x.lo);
+}
+
 // A stream's first token, the number of its tokens and the rows of its cache that count (-1: outside the table).
 struct Stream {
   int first, n, kv;
 };
 
 __device__ __forceinline__ Stream stream_at(const Batch& a, int b) {
-  const int64_t c0 = idx_at(a.cu, a.i64, b), c1 = idx_at(a.cu, a.i64, b + 1);
+  const Index i0 = index_at(a.cu, a.i64, b), i1 = index_at(a.cu, a.i64, b + 1);
+  const Index ik = index_at(a.lens ? a.lens : a.cu, a.i64, b);
+  const int64_t c0 = value_of(i0, a.i64), c1 = value_of(i1, a.i64), kv = value_of(ik, a.i64);
   Stream s;
   s.first = static_cast<int>(min(max(c0, static_cast<int64_t>(0)), static_cast<int64_t>(a.tokens)));
   s.n = static_cast<int>(min(max(c1, static_cast<int64_t>(s.first)), static_cast<int64_t>(a.tokens))) - s.first;
-  if (a.lens) {
-    const int64_t kv = idx_at(a.lens, a.i64, b);
-    s.kv = kv < 0 || kv > a.max_keys ? -1 : static_cast<int>(kv);
-  } else {
-    s.kv = s.n;  // a prompt's own rows
-  }
+  s.kv = !a.lens ? s.n : kv < 0 || kv > a.max_keys ? -1 : static_cast<int>(kv);  // no lengths: a prompt's own rows
   return s;
 }
 
@@ -170,18 +183,15 @@ __device__ __forceinline__ int pieces_of(int keys, int cut) {
   return cut == 0 ? 1 : max(1, (g + cut - 1) / cut);
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int o = __shfl_up(v, d, kWave);
-    v += lane_id() >= d ? o : 0;
-  }
-  return v;
-}
-
-__device__ __forceinline__ int64_t wave_total(int64_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
+// Inclusive prefix sums over the wave: within rows of 16 lanes, then rows 0 and 2 into 1 and 3, then lane 31 into the
+// upper half.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
 
@@ -198,13 +208,14 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
   };
   load(0);
   if (a.target > 0) {
-    int64_t total = 0;
+    double total = 0.;  // exact in each lane below 2^53
     for (int base = 0; base < B; base += kWave) {
       if (base) load(base);
-      total += static_cast<int64_t>(blocks_of<BR>(mine, G)) * ((max(mine.kv, 0) + GR - 1) / GR);
+      total += static_cast<double>(blocks_of<BR>(mine, G)) * ((max(mine.kv, 0) + GR - 1) / GR);
     }
-    total = wave_total(total);
-    k.cut = static_cast<int>(max((total + a.target - 1) / a.target, static_cast<int64_t>(1)));
+    // rounded up by more than the sum over the lanes can lose, so that cut keeps the pieces within target
+    const float pieces = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / a.target);
+    k.cut = static_cast<int>(fminf(fmaxf(pieces, 1.f), 1073741824.f));
     if (B > kWave) load(0);
   }
   int slots = 0;
@@ -275,26 +286,25 @@ struct Mfma<FP16> {
   static constexpr uint32_t kExp = 0x7c007c00u;
 };
 
-// Whether a pair of values holds an infinity or a NaN.
+// acc & kNotFinite says whether some pair accumulated by add_exponents held an infinity or a NaN: an exponent
+// of ones and no other carries into its half's top bit.
 template <class T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t lo = Mfma<T>::kExp & 0xffffu, hi = Mfma<T>::kExp & 0xffff0000u;
-  return (w & lo) == lo || (w & hi) == hi;
+__device__ __forceinline__ uint32_t add_exponents(uint32_t acc, uint32_t w) {
+  constexpr uint32_t one = Mfma<T>::kExp & (~Mfma<T>::kExp << 1);  // the exponents' last bits
+  return acc | ((w & Mfma<T>::kExp) + one);
+}
+template <class T>
+__device__ __forceinline__ uint32_t add_exponents(uint32_t acc, const uint4& w) {
+  return add_exponents<T>(add_exponents<T>(add_exponents<T>(add_exponents<T>(acc, w.x), w.y), w.z), w.w);
+}
+constexpr uint32_t kNotFinite = 0x80008000u;
+
+// The page number of a key.
+__device__ __forceinline__ Index page_id(const AttnArgs& a, int b, int key) {
+  return index_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + div_by(key, a.page));
 }
 
-// The page number read for a key, as it came (both halves of a 64-bit entry; the same word twice of a 32-bit one), so
-// that nothing waits for it before it is used.
-struct PageId {
-  uint32_t lo, hi;
-};
-
-__device__ __forceinline__ PageId page_id(const AttnArgs& a, int b, int key) {
-  const int64_t i = b * a.batch.table_stride + div_by(key, a.page);
-  const uint32_t* p = static_cast<const uint32_t*>(a.batch.table) + (a.batch.i64 ? 2 * i : i);
-  return PageId{p[0], p[a.batch.i64 ? 1 : 0]};
-}
-
-__device__ __forceinline__ bool page_ok(const AttnArgs& a, PageId id) {
+__device__ __forceinline__ bool page_ok(const AttnArgs& a, Index id) {
   return static_cast<int>(id.lo) >= 0 && static_cast<int>(id.lo) < a.n_pages && (!a.batch.i64 || id.hi == 0);
 }
 
@@ -322,7 +332,7 @@ __device__ __forceinline__ RowSums row_by_keys(const AttnArgs& a, const Work& w,
     bool ok = k0 + lane < end;
     const uint16_t *kr, *vr;
     if (a.batch.table) {
-      const PageId id = page_id(a, w.b, key);
+      const Index id = page_id(a, w.b, key);
       ok = ok && page_ok(a, id);
       const int at = key - static_cast<int>(div_by(key, a.page)) * static_cast<int>(a.page.d);
       kr = a.kp.at(static_cast<int>(id.lo), kvh, at);

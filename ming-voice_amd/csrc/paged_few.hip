@@ -84,7 +84,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   // the rows of a tile's keys: lane l's key and value row, and which of the 32 exist
   const char *kr, *vr;
   uint32_t there = 0;
-  auto find_rows = [&](int it, PageId id) {
+  auto find_rows = [&](int it, Index id) {
     const int key = k_begin + it * kKeys + (lane & (kKeys - 1));
     bool ok = key < k_end;
     const int kc = min(key, k_end - 1);
@@ -153,9 +153,9 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
     for (int nt = 0; nt < NT; ++nt) o[f][nt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   const float sc = a.scale * 1.4426950408889634f;  // scores in units of log2: exp2 gives the weights
-  bool bad = false;
+  uint32_t seen = 0;  // exponents of values that some row must not meet
   if (wave < tiles) {
-    PageId next{0, 0};
+    Index next{0, 0};
     if constexpr (PAGED) next = page_id(a, w.b, key_of(wave));
     find_rows(wave, next);
     if constexpr (PAGED) next = page_id(a, w.b, key_of(wave + NW));
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
         for (int b = 0; b < 4; ++b) {
           const uint4 vf = make_uint4(static_cast<uint32_t>(lo[b]), static_cast<uint32_t>(lo[b] >> 32),
                                       static_cast<uint32_t>(hi[b]), static_cast<uint32_t>(hi[b] >> 32));
-          if (mixed) bad = bad || not_finite<T>(vf.x) || not_finite<T>(vf.y) || not_finite<T>(vf.z) || not_finite<T>(vf.w);
+          if (mixed) seen = add_exponents<T>(seen, vf);
 #pragma unroll
           for (int f = 0; f < QF; ++f) o[f][n0 + b] = Mfma<T>::m16(vf, pf[f], o[f][n0 + b]);
         }
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
       so[P::ML + BR + 16 * f + lr] = l[f];
     }
   }
-  const bool mine_met = __any(bad);
+  const bool mine_met = __any((seen & kNotFinite) != 0);
   if (lane == 0) so[P::MET] = mine_met ? 1.f : 0.f;
   __syncthreads();
   float* state = pieces > 1 ? state_at<BR>(a, w.slot + w.piece, kvh) : nullptr;
@@ -373,6 +373,57 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   }
 }
 
+// The same for blocks of many rows, which are cut into few pieces: dv / 4 lanes to a row, each through all pieces. Grid (cut
+// blocks, key / value heads, BR / ROWS) x 256.
+template <class T, int BR, int GR, int ROWS>
+__global__ __launch_bounds__(256) void join_rows_kernel(AttnArgs a) {
+  const int tid = threadIdx.x, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
+  const Work w = scalars(find_work<BR, GR, true>(a, blockIdx.x));
+  if (w.b < 0) return;
+  const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<GR>(keys, w.cut);
+  if (pieces == 1) return;
+  const int n4 = a.dv / 4, at_once = 256 / n4, rows = min(BR, w.s.n * G - w.blk * BR);
+  const int my = tid / n4, d = 4 * (tid - my * n4);
+  const float* first = state_at<BR>(a, w.slot, kvh);
+  const int64_t step = static_cast<int64_t>(a.nkv) * BR * (a.dv + 2);
+  const int end = min(rows, static_cast<int>(blockIdx.z) * ROWS + ROWS);
+  if (my >= at_once) return;
+  for (int r = static_cast<int>(blockIdx.z) * ROWS + my; r < end; r += at_once) {
+    float m = -INFINITY, l = 0.f;
+    floatx4 acc = floatx4{0.f, 0.f, 0.f, 0.f};
+    constexpr int kAtOnce = 4;
+    for (int p = 0; p < pieces; p += kAtOnce) {
+      float pm[kAtOnce], pl[kAtOnce];
+      floatx4 pa[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const float* s = first + min(p + u, pieces - 1) * step;
+        pm[u] = s[BR * a.dv + r];
+        pl[u] = s[BR * a.dv + BR + r];
+        pa[u] = *reinterpret_cast<const floatx4*>(s + r * a.dv + d);
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) mn = fmaxf(mn, p + u < pieces ? pm[u] : -INFINITY);
+      const float mu = mn == -INFINITY ? 0.f : mn, alpha = exp2_fast(m - mu);
+      m = mn;
+      l *= alpha;
+      acc *= alpha;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (p + u < pieces) {
+          const float wt = exp2_fast(pm[u] - mu);
+          l = fmaf(pl[u], wt, l);
+          acc += wt * pa[u];
+        }
+    }
+    const int row = w.blk * BR + r, i = static_cast<int>(div_by(row, a.group));
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(a.out.at(w.s.first + i, kvh * G + (row - i * G)) + d) =
+        make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+  }
+}
+
 template <class T, int BR, int GR, int ROWS, int RW>
 int launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
   hipLaunchKernelGGL((join_kernel<T, BR, GR, ROWS, RW>),
@@ -420,7 +471,11 @@ int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipS
 }
 
 int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what) {
-  return dtype == MM_BF16 ? launch_join<BF16, 128, 64, 32, 4>(a, p, st, what) : launch_join<FP16, 128, 64, 32, 4>(a, p, st, what);
+  constexpr int ROWS = 16;
+  const dim3 grid(static_cast<unsigned>(p.blocks < p.target ? p.blocks : p.target), static_cast<unsigned>(a.nkv), 128 / ROWS);
+  if (dtype == MM_BF16) hipLaunchKernelGGL((join_rows_kernel<BF16, 128, 64, ROWS>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((join_rows_kernel<FP16, 128, 64, ROWS>), grid, dim3(256), 0, st, a);
+  return mm::check_launch(what);
 }
 
 }  // namespace mmp

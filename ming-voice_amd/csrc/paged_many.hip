@@ -93,10 +93,16 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
   // the page numbers of a tile: of key l (kAnywhere), of keys 8 (l % 8) .. + 7 (kPaged)
   auto ids_of = [&](int it) {
     const int key = k_begin + it * kKeys + (SRC == kAnywhere ? lane : 8 * (lane % 8));
-    if (SRC == kPacked || (SRC == kAnywhere && !a.batch.table)) return PageId{0, 0};
+    if (SRC == kPacked || (SRC == kAnywhere && !a.batch.table)) return Index{0, 0};
     return page_id(a, w.b, min(key, k_end - 1));
   };
-  auto load_tile = [&](int it, PageId id, char* kt, char* vt) {
+  const char *kpk = nullptr, *vpk = nullptr;  // kPacked: the wave's first row of the tile to load
+  if constexpr (SRC == kPacked) {
+    kpk = reinterpret_cast<const char*>(a.k.at(w.s.first + k_begin + 8 * wave, kvh));
+    vpk = reinterpret_cast<const char*>(a.v.at(w.s.first + k_begin + 8 * wave, kvh));
+  }
+  const uint32_t kfull = 7 * krs + 2 * a.dqk, vfull = 7 * vrs + 2 * a.dv;  // 8 rows
+  auto load_tile = [&](int it, Index id, char* kt, char* vt) {
     const int j0 = k_begin + it * kKeys, left = k_end - j0;  // keys of the tile and behind
     if constexpr (SRC == kAnywhere) {
       const int key = min(j0 + lane, k_end - 1);
@@ -135,24 +141,29 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
 #pragma unroll
         for (int s = 0; s < VS; ++s) load_lds16(vdim + 64 * s < a.dv ? vp + 128 * s : zeros, vd + s * P::PIECE);
       } else {
-        const int n = min(8, static_cast<int>(__popcll(there & (0xffull << r))));  // its rows that exist, the first ones
-        const uint16_t *kb, *vb;
+        int n = min(8, max(0, left - r));  // its rows that exist
+        const char *kb, *vb;
         if constexpr (SRC == kPaged) {
-          const int page = n ? __builtin_amdgcn_readlane(static_cast<int>(id.lo), 4 * i + wave) : 0;
+          const int page = __builtin_amdgcn_readlane(static_cast<int>(id.lo), 4 * i + wave);
           const int row = (j0 + r) - static_cast<int>(div_by(j0 + r, a.page)) * static_cast<int>(a.page.d);
-          kb = a.kp.at(page, kvh, row);
-          vb = a.vp.at(page, kvh, row);
+          if (!((there >> r) & 1)) n = 0;
+          kb = reinterpret_cast<const char*>(a.kp.at(n ? page : 0, kvh, row));
+          vb = reinterpret_cast<const char*>(a.vp.at(n ? page : 0, kvh, row));
         } else {
-          kb = a.k.at(w.s.first + j0 + r, kvh);
-          vb = a.v.at(w.s.first + j0 + r, kvh);
+          kb = kpk + 32 * i * static_cast<int64_t>(krs);
+          vb = vpk + 32 * i * static_cast<int64_t>(vrs);
         }
-        const rsrc_t kres = make_rsrc(kb, n ? (n - 1) * static_cast<int64_t>(krs) + 2 * a.dqk : 0);
-        const rsrc_t vres = make_rsrc(vb, n ? (n - 1) * static_cast<int64_t>(vrs) + 2 * a.dv : 0);
+        const uint32_t kbytes = n == 8 ? kfull : n ? (n - 1) * krs + 2 * a.dqk : 0, vbytes = n == 8 ? vfull : n ? (n - 1) * vrs + 2 * a.dv : 0;
+        const rsrc_t kres = make_rsrc(kb, kbytes), vres = make_rsrc(vb, vbytes);
 #pragma unroll
         for (int s = 0; s < KS; ++s) buf_lds16(kres, kdim + 64 * s < a.dqk ? koff + 128u * s : kPast, kd + s * P::PIECE);
 #pragma unroll
         for (int s = 0; s < VS; ++s) buf_lds16(vres, vdim + 64 * s < a.dv ? voff + 128u * s : kPast, vd + s * P::PIECE);
       }
+    }
+    if constexpr (SRC == kPacked) {
+      kpk += 64 * static_cast<int64_t>(krs);
+      vpk += 64 * static_cast<int64_t>(vrs);
     }
   };
 
@@ -190,15 +201,15 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   const float sc = a.scale * 1.4426950408889634f;
 
-  bool bad = false;
-  PageId next{0, 0};
+  uint32_t seen = 0;  // exponents of values that some row must not meet
+  Index next{0, 0};
   auto tile = [&](int it, char* kt, char* vt, char* kt_next, char* vt_next) {
     const int j0 = k_begin + it * kKeys;
     const uint64_t mine = there;
     wait_vmcnt<0>();  // this wave's part of the tile
     __syncthreads();  // every wave's part; and the other buffer has been read
     if (it + 1 < tiles) {
-      const PageId id = next;
+      const Index id = next;
       next = ids_of(it + 2);
       load_tile(it + 1, id, kt_next, vt_next);
     }
@@ -208,7 +219,7 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
 #pragma unroll
         for (int s = 0; s < VS; ++s) {
           const uint4 x = *reinterpret_cast<const uint4*>(vt + s * P::PIECE + (32 * i + 8 * wave) * 128 + lane * 16);
-          bad = bad || not_finite<T>(x.x) || not_finite<T>(x.y) || not_finite<T>(x.z) || not_finite<T>(x.w);
+          seen = add_exponents<T>(seen, x);
         }
     }
     if (j0 < lim_max) {
@@ -217,13 +228,32 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+      constexpr int AHEAD = KS <= 2 ? NK : 4;  // k steps whose fragments are read before the first product
 #pragma unroll
-      for (int ks = 0; ks < NK; ++ks)
+      for (int k0 = 0; k0 < NK; k0 += AHEAD) {
+        uint4 kx[2][AHEAD];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + (ks / 4) * P::PIECE + u * 4096 + (kplace ^ (32 * (ks % 4))));
-          s[u] = Mfma<T>::m32(x, qf[ks], s[u]);
-        }
+        for (int ks = 0; ks < AHEAD; ++ks)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            kx[u][ks] = *reinterpret_cast<const uint4*>(kt + ((k0 + ks) / 4) * P::PIECE + u * 4096 + (kplace ^ (32 * (ks % 4))));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < AHEAD; ++ks)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s[u] = Mfma<T>::m32(kx[u][ks], qf[k0 + ks], s[u]);
+      }
+      // the value fragments too, before the softmax (where they fit: 8 KB a tile and 64 dims, 4 registers a fragment)
+      constexpr bool EARLY = KS <= 3;
+      uint4 vf[4][ND];
+      if constexpr (EARLY) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt)
+            vf[st][dt] = v_frag(vt + (dt / 2) * P::PIECE + (vplace ^ (64 * (dt % 2))) + 16 * st * 128, 8 * 128);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       uint64_t sees = ~0ull;
       if (j0 + kKeys > lim_min || mine != ~0ull) {  // s[u][i]: key 32 u + 8 (i / 4) + 4 lh + i % 4
         const int n = lim - j0;
@@ -264,12 +294,14 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
 #pragma unroll
       for (int st = 0; st < 4; ++st)
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-          o[dt] = Mfma<T>::m32(v_frag(vt + (dt / 2) * P::PIECE + (vplace ^ (64 * (dt % 2))) + 16 * st * 128, 8 * 128), pf[st], o[dt]);
+        for (int dt = 0; dt < ND; ++dt) {
+          if constexpr (!EARLY) vf[st][dt] = v_frag(vt + (dt / 2) * P::PIECE + (vplace ^ (64 * (dt % 2))) + 16 * st * 128, 8 * 128);
+          o[dt] = Mfma<T>::m32(vf[st][dt], pf[st], o[dt]);
+        }
     }
   };
   if (tiles > 0) {
-    const PageId id = ids_of(0);
+    const Index id = ids_of(0);
     next = ids_of(1);
     load_tile(0, id, s_k0, s_v0);
   }
@@ -281,7 +313,7 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
   // whether any wave met such a value: in words of the key buffer, which is no longer needed
   __syncthreads();
   int* met = reinterpret_cast<int*>(s_k0);
-  const bool mine_met = __any(bad);
+  const bool mine_met = __any((seen & kNotFinite) != 0);
   if (lane == 0) met[wave] = mine_met;
   __syncthreads();
   if (__builtin_amdgcn_readfirstlane(met[0] | met[1] | met[2] | met[3])) {
