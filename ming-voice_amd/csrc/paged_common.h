@@ -107,11 +107,23 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
   }
 }
 
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// Two values rounded to nearest even, side by side: one instruction (converted one by one they take four).
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (T::kBf16) return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
-  else return static_cast<uint32_t>(f32_to_f16(lo)) | (static_cast<uint32_t>(f32_to_f16(hi)) << 16);
+  if constexpr (T::kBf16) {
+    const bf16x2_t v = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    const f16x2_t v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  }
 }
+
+// The larger, NaN where either is: one v_maximum3 for two of them, where fmaxf first quiets each operand that does not
+// come out of an arithmetic instruction.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 template <class T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
@@ -152,15 +164,14 @@ struct AttnArgs {
 
 // How the work is divided. A row is one token's query at one of the G heads that share a key / value head (row r of a
 // stream: token r / G, head r % G), so that a block of BR rows reads each key once for all of them. A stream of n tokens
-// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys are cut into pieces of `cut` granules of GR keys:
-// cut is the smallest for which the sum over all blocks of (granules / cut) stays within target, so the pieces are of one
-// length whatever the streams' lengths are, and a long stream among short ones is shared by many workgroups. Only blocks
-// of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there are at most 2 target of them, a bound that needs
-// no length on the host. Workgroups are at most target + blocks.
+// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys may be cut into pieces of `cut` granules of GR keys,
+// one cut for the whole batch, so that a long stream among short ones is shared by many workgroups. cut is at least the sum
+// over all blocks of (granules / target). Only blocks of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there
+// are at most 2 target of them, a bound that needs no length on the host, as workgroups are at most target + blocks.
 struct Work {
   int b, blk;      // stream (-1: none) and row block
   int piece;       // of the block's keys
-  int cut;         // granules in a piece
+  int cut;         // granules in a piece (0: all)
   int slot;        // state of the block's first piece
   Stream s;
 };
@@ -195,6 +206,22 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// The granules of a piece: as many pieces as target allows; of many rows (a piece pays for its state of BR rows and the
+// join) kMinCut granules at least.
+constexpr int kMinCut = 4;
+
+template <int BR, int GR, class Load>
+__device__ __forceinline__ int cut_of(const AttnArgs& a, const Stream& mine, Load load) {
+  double total = 0.;  // exact in each lane below 2^53
+  for (int base = 0; base < a.batch.seqs; base += kWave) {
+    if (base) load(base);
+    total += static_cast<double>(blocks_of<BR>(mine, static_cast<int>(a.group.d))) * ((max(mine.kv, 0) + GR - 1) / GR);
+  }
+  // rounded up by more than the sum over the lanes can lose, so that no cut gives more pieces than target
+  const float cut = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / static_cast<float>(a.target));
+  return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), 1073741824.f));
+}
+
 // The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the batch itself: streams 64 at a
 // time, one to a lane. Within a stream the last row block, whose rows see the most keys, comes first.
 template <int BR, int GR, bool CUT>
@@ -208,14 +235,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
   };
   load(0);
   if (a.target > 0) {
-    double total = 0.;  // exact in each lane below 2^53
-    for (int base = 0; base < B; base += kWave) {
-      if (base) load(base);
-      total += static_cast<double>(blocks_of<BR>(mine, G)) * ((max(mine.kv, 0) + GR - 1) / GR);
-    }
-    // rounded up by more than the sum over the lanes can lose, so that cut keeps the pieces within target
-    const float pieces = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / a.target);
-    k.cut = static_cast<int>(fminf(fmaxf(pieces, 1.f), 1073741824.f));
+    k.cut = cut_of<BR, GR>(a, mine, load);
     if (B > kWave) load(0);
   }
   int slots = 0;
@@ -399,13 +419,17 @@ __device__ __forceinline__ void rows_by_keys(const AttnArgs& a, const Work& w, i
   }
 }
 
-// What a call launches. Few rows to a block (16) or many (128); target: pieces of keys aimed at for the whole batch (0: no
-// cutting, no join); blocks: the most row blocks that these sizes can have.
+// What a call launches, a function of its sizes alone. Few rows to a block (16) or many (128); target: pieces of keys aimed
+// at for the whole batch and one key / value head (0: no cutting, no join); blocks: the most row blocks that these sizes
+// can have.
 struct AttnPlan {
   bool many;
+  int groups;  // of four waves in a workgroup of many rows
   int64_t blocks, target, workspace;
 };
-AttnPlan plan_attn(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+// The most workspace that a call of at most these tokens, streams and keys takes.
+int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
 int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
 int launch_many(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
 int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what);

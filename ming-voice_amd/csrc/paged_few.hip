@@ -202,7 +202,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
         for (int e = 0; e < 8; ++e) {  // slot e < 4 is key 4 lq + e of the tile, slot e >= 4 key 16 + 4 lq + e - 4
           const bool see = e < 4 ? (lo4 >> e) & 1u : (hi4 >> (e - 4)) & 1u;
           sv[e] = see ? (e < 4 ? s[f][0][e] : s[f][1][e - 4]) * sc : -INFINITY;
-          tmax = fmaxf(tmax, sv[e]);
+          tmax = larger(tmax, sv[e]);
         }
         const float mn = fmaxf(m[f], quarter_max(tmax));
         const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
@@ -453,15 +453,25 @@ int launch_type(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char
 
 }  // namespace
 
-AttnPlan plan_attn(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
   AttnPlan p{};
-  const int64_t rows = tokens * (nh / nkv);
-  p.many = rows > 16 * seqs;  // more than 16 rows a stream on average
-  const int64_t br = p.many ? 128 : 16, gr = p.many ? 64 : (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys;
-  p.blocks = rows / br + seqs < rows ? rows / br + seqs : rows;
-  if (max_keys > gr) p.target = (2 * mm::cu_count() + nkv - 1) / nkv;
-  p.workspace = 2 * p.target * nkv * br * (dv + 2) * 4;
+  const int64_t rows = tokens * (nh / nkv), cus = mm::cu_count();
+  auto blocks_of = [&](int64_t br) { return rows / br + seqs < rows ? rows / br + seqs : rows; };
+  const int64_t reads = blocks_of(16) * nkv * max_keys * (dqk + dv) * 2;
+  p.many = rows > 16 * seqs && reads > (64LL << 20);
+  p.blocks = blocks_of(p.many ? 128 : 16);
+  if (p.many) {
+    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus) p.target = (2 * cus + nkv - 1) / nkv;
+    p.groups = !paged && p.target == 0 && p.blocks * nkv < 4 * cus ? 2 : 1;
+  } else if (max_keys > 4 * (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys) {
+    p.target = (4 * cus + nkv - 1) / nkv;
+  }
+  p.workspace = 2 * p.target * nkv * (p.many ? 128 : 16) * (dv + 2) * 4;
   return p;
+}
+
+int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
+  return plan_attn(paged, tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
 }
 
 int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {

@@ -200,17 +200,13 @@ void set_pool(const mm_pages* g, Pool& k, Pool& v) {
   v = Pool{static_cast<uint16_t*>(g->v), g->v_page_stride, g->v_head_stride, g->v_row_stride};
 }
 
-int64_t workspace_of(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
-  return plan_attn(tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
-}
-
 int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int64_t workspace_bytes, hipStream_t st,
            const char* what) {
   const int64_t max_keys = paged ? a.batch.max_keys : a.batch.tokens;
   // 0 would turn the -infinity of a key that is not seen into NaN; this leaves every finite score at zero
   a.scale = scale == 0.f ? 1e-37f : fabsf(scale);
   a.negative = scale < 0.f;
-  const AttnPlan p = plan_attn(a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
+  const AttnPlan p = plan_attn(paged, a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
   MM_REQUIRE((p.blocks + p.target) * a.nkv <= 0x7fffffff, "%s: too many rows", what);
   MM_REQUIRE(p.workspace == 0 || (workspace && mm::aligned16(workspace) && workspace_bytes >= p.workspace),
              "%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)p.workspace);
@@ -272,7 +268,7 @@ extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t
   if (check_shape("paged_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("paged_attn", tokens, seqs) || max_keys < 0 ||
       max_keys > kMaxKeys)
     return -1;
-  return workspace_of(tokens, seqs, max_keys, nh, nkv, dqk, dv);
+  return workspace_of(true, tokens, seqs, max_keys, nh, nkv, dqk, dv);
 }
 
 extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
@@ -301,7 +297,7 @@ extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, 
 
 extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv) {
   if (check_shape("prompt_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("prompt_attn", tokens, seqs)) return -1;
-  return workspace_of(tokens, seqs, tokens, nh, nkv, dqk, dv);
+  return workspace_of(false, tokens, seqs, tokens, nh, nkv, dqk, dv);
 }
 
 extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,

@@ -7,18 +7,19 @@ namespace mmp {
 namespace {
 
 constexpr int kKeys = 64;   // keys per tile
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;    // waves of a group: one group shares a tile
 constexpr int kRows = 32;   // rows per wave
 
 // The shape of many_kernel: head dims up to 64 KS (q, k) and 64 VS (v). A tile lies in LDS as pieces of 64 keys by 64 dims,
 // 8 KB each: every load instruction then fills 8 rows of 128 bytes, whatever the head dims are.
-template <int KS, int VS>
+template <int KS, int VS, int NG>
 struct Many {
   static constexpr int BR = kWaves * kRows;
+  static constexpr int THREADS = NG * kWaves * kWave;
   static constexpr int GR = kKeys;
   static constexpr int PIECE = kKeys * 128;  // bytes
   static constexpr int K_BYTES = KS * PIECE, V_BYTES = VS * PIECE;
-  static_assert(2 * (K_BYTES + V_BYTES) <= 159 * 1024, "tile shape");
+  static_assert(2 * NG * (K_BYTES + V_BYTES) <= 160 * 1024, "tile shape");
 };
 
 // The chunk of a piece's row held at LDS place c of the row (involutions). Keys: the 16 rows that a fragment reads at one
@@ -40,20 +41,20 @@ __device__ __forceinline__ uint4 v_frag(const char* p, int hi) {
 // Max over the two lanes that share lane % 32.
 __device__ __forceinline__ float half_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), true, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Where a tile's rows come from, chosen on the host (rows_of_kind).
 enum Source { kPacked, kPaged, kAnywhere };
 
-template <class T, int KS, int VS, int SRC>
-__global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(AttnArgs a) {
-  using P = Many<KS, VS>;
+template <class T, int KS, int VS, int NG, int SRC>
+__global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(AttnArgs a) {
+  using P = Many<KS, VS, NG>;
   constexpr int BR = P::BR, NK = 4 * KS, ND = 2 * VS;
   // two buffers, each an object of its own: reads of one then need not wait for the loads in flight into the other
-  __shared__ __align__(1024) char s_k0[P::K_BYTES], s_v0[P::V_BYTES], s_k1[P::K_BYTES], s_v1[P::V_BYTES];
+  __shared__ __align__(1024) char s_k0[NG * P::K_BYTES], s_v0[NG * P::V_BYTES], s_k1[NG * P::K_BYTES], s_v1[NG * P::V_BYTES];
   const int tid = threadIdx.x, lane = lane_id();
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int all_wave = __builtin_amdgcn_readfirstlane(tid / kWave), wave = all_wave % kWaves, group = all_wave / kWaves;
   const int lr = lane & 31, lh = lane >> 5, G = static_cast<int>(a.group.d);
   const int unit = static_cast<int>(blockIdx.x) / a.nkv, kvh = static_cast<int>(blockIdx.x) - unit * a.nkv;
   const Work w = scalars(find_work<BR, P::GR, false>(a, unit));
@@ -64,14 +65,14 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
     return a.out.at(w.s.first + i, kvh * G + (r0 + r - i * G));
   };
   if (w.s.kv < 0) {
-    for (int i = tid; i < rows * a.dv; i += kWaves * kWave) T::st(out_at(i / a.dv), i % a.dv, NAN);
+    for (int i = tid; i < rows * a.dv; i += P::THREADS) T::st(out_at(i / a.dv), i % a.dv, NAN);
     return;
   }
   const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<P::GR>(keys, w.cut);
   if (w.piece >= pieces) return;
   const int k_begin = w.piece * w.cut * P::GR;
   const int k_end = w.cut == 0 ? keys : min(keys, k_begin + w.cut * P::GR);
-  const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;
+  const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;  // group g takes tiles g, g + NG, ..
   const int ctx = w.s.kv - w.s.n;
 
   // A wave fills rows 8 wave .. + 7 and 32 + 8 wave .. + 7 of each piece, lane l row l / 8 of them at LDS place l % 8.
@@ -98,8 +99,8 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
   };
   const char *kpk = nullptr, *vpk = nullptr;  // kPacked: the wave's first row of the tile to load
   if constexpr (SRC == kPacked) {
-    kpk = reinterpret_cast<const char*>(a.k.at(w.s.first + k_begin + 8 * wave, kvh));
-    vpk = reinterpret_cast<const char*>(a.v.at(w.s.first + k_begin + 8 * wave, kvh));
+    kpk = reinterpret_cast<const char*>(a.k.at(w.s.first + k_begin + kKeys * group + 8 * wave, kvh));
+    vpk = reinterpret_cast<const char*>(a.v.at(w.s.first + k_begin + kKeys * group + 8 * wave, kvh));
   }
   const uint32_t kfull = 7 * krs + 2 * a.dqk, vfull = 7 * vrs + 2 * a.dv;  // 8 rows
   auto load_tile = [&](int it, Index id, char* kt, char* vt) {
@@ -162,8 +163,8 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
       }
     }
     if constexpr (SRC == kPacked) {
-      kpk += 64 * static_cast<int64_t>(krs);
-      vpk += 64 * static_cast<int64_t>(vrs);
+      kpk += NG * kKeys * static_cast<int64_t>(krs);
+      vpk += NG * kKeys * static_cast<int64_t>(vrs);
     }
   };
 
@@ -208,11 +209,12 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
     const uint64_t mine = there;
     wait_vmcnt<0>();  // this wave's part of the tile
     __syncthreads();  // every wave's part; and the other buffer has been read
-    if (it + 1 < tiles) {
+    if (it + NG < tiles) {
       const Index id = next;
-      next = ids_of(it + 2);
-      load_tile(it + 1, id, kt_next, vt_next);
+      next = ids_of(it + 2 * NG);
+      load_tile(it + NG, id, kt_next, vt_next);
     }
+    if (NG > 1 && it >= tiles) return;  // the other group's last tile
     if (j0 + kKeys > lim_block) {  // some row does not see some key: its value must be finite, or 0 * inf reaches the row
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -265,9 +267,9 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
           for (int i = 0; i < 16; ++i) s[u][i] = (bits >> (8 * (i / 4) + i % 4)) & 1u ? s[u][i] : -INFINITY;
         }
       }
-      float tmax = fmaxf(s[0][0], s[1][0]);
+      float tmax = larger(s[0][0], s[1][0]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, fmaxf(s[0][i], s[1][i]));
+      for (int i = 1; i < 16; ++i) tmax = larger(larger(tmax, s[0][i]), s[1][i]);
       tmax = half_max(tmax);
       if (__any((tmax - m) * sc > 8.f)) {  // the sums stay below 2^8 of a weight of one: no need to follow every rise
         const float mn = fmaxf(m, tmax), mu = mn == -INFINITY ? 0.f : mn;
@@ -300,28 +302,61 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
         }
     }
   };
-  if (tiles > 0) {
-    const Index id = ids_of(0);
-    next = ids_of(1);
-    load_tile(0, id, s_k0, s_v0);
+  char *k0 = s_k0 + group * P::K_BYTES, *v0 = s_v0 + group * P::V_BYTES, *k1 = s_k1 + group * P::K_BYTES, *v1 = s_v1 + group * P::V_BYTES;
+  if (group < tiles) {
+    const Index id = ids_of(group);
+    next = ids_of(group + NG);
+    load_tile(group, id, k0, v0);
   }
-  for (int it = 0; it < tiles; it += 2) {
-    tile(it, s_k0, s_v0, s_k1, s_v1);
-    if (it + 1 < tiles) tile(it + 1, s_k1, s_v1, s_k0, s_v0);
+  for (int it = 0; it < tiles; it += 2 * NG) {
+    tile(it + group, k0, v0, k1, v1);
+    if (it + NG < tiles) tile(it + NG + group, k1, v1, k0, v0);
   }
   float* state = pieces > 1 ? state_at<BR>(a, w.slot + w.piece, kvh) : nullptr;
   // whether any wave met such a value: in words of the key buffer, which is no longer needed
   __syncthreads();
   int* met = reinterpret_cast<int*>(s_k0);
   const bool mine_met = __any((seen & kNotFinite) != 0);
-  if (lane == 0) met[wave] = mine_met;
+  if (lane == 0) met[all_wave] = mine_met;
   __syncthreads();
-  if (__builtin_amdgcn_readfirstlane(met[0] | met[1] | met[2] | met[3])) {
-    rows_by_keys<T, BR>(a, w, kvh, rows, wave, kWaves, k_begin, k_end, state);
+  int any_met = 0;
+#pragma unroll
+  for (int x = 0; x < NG * kWaves; ++x) any_met |= met[x];
+  if (__builtin_amdgcn_readfirstlane(any_met)) {
+    rows_by_keys<T, BR>(a, w, kvh, rows, all_wave, NG * kWaves, k_begin, k_end, state);
     return;
   }
-  if (lr >= wrows) return;
   l += __shfl_xor(l, 32, kWave);
+  if constexpr (NG == 2) {
+    // the second group's state to the first, a fragment's register of all lanes side by side: 16 KB of sums per 32 dims,
+    // the first in one buffer, the rest in the other
+    constexpr int HALF = ND / 2;
+    static_assert(HALF * 16 * 1024 <= NG * P::V_BYTES, "room");
+    __syncthreads();
+    float* ml = reinterpret_cast<float*>(s_k0) + wave * 2 * kWave + lane;
+    auto sums = [&](int dt) {
+      return reinterpret_cast<float*>(dt < HALF ? s_v0 : s_v1) + ((dt % HALF) * kWaves + wave) * 16 * kWave + lane;
+    };
+    if (group == 1) {
+      ml[0] = m;
+      ml[kWave] = l;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums(dt)[i * kWave] = o[dt][i];
+    }
+    __syncthreads();
+    if (group == 1) return;
+    const float m1 = ml[0], mn = fmaxf(m, m1), mu = mn == -INFINITY ? 0.f : mn;
+    const float a0 = exp2_fast((m - mu) * sc), a1 = exp2_fast((m1 - mu) * sc);
+    m = mn;
+    l = l * a0 + ml[kWave] * a1;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] = fmaf(sums(dt)[i * kWave], a1, o[dt][i] * a0);
+  }
+  if (lr >= wrows) return;
   const int r = kRows * wave + lr;  // of the workgroup
   if (state) {
 #pragma unroll
@@ -349,19 +384,24 @@ __global__ __launch_bounds__(kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(A
     }
 }
 
-template <class T, int KS, int VS, int SRC>
+template <class T, int KS, int VS, int NG, int SRC>
 int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL((many_kernel<T, KS, VS, SRC>), dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)),
-                     dim3(kWaves * kWave), 0, st, a);
+  hipLaunchKernelGGL((many_kernel<T, KS, VS, NG, SRC>), dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)),
+                     dim3(NG * kWaves * kWave), 0, st, a);
   return mm::check_launch(what);
+}
+
+template <class T, int KS, int VS, int SRC>
+int launch_groups(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
+  return p.groups == 2 ? launch_shape<T, KS, VS, 2, SRC>(a, p, st, what) : launch_shape<T, KS, VS, 1, SRC>(a, p, st, what);
 }
 
 template <class T, int SRC>
 int launch_source(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  if (a.dqk <= 64 && a.dv <= 64) return launch_shape<T, 1, 1, SRC>(a, p, st, what);
-  if (a.dqk <= 128 && a.dv <= 128) return launch_shape<T, 2, 2, SRC>(a, p, st, what);
-  if (a.dqk <= 192 && a.dv <= 128) return launch_shape<T, 3, 2, SRC>(a, p, st, what);
-  return launch_shape<T, 4, 4, SRC>(a, p, st, what);
+  if (a.dqk <= 64 && a.dv <= 64) return launch_groups<T, 1, 1, SRC>(a, p, st, what);
+  if (a.dqk <= 128 && a.dv <= 128) return launch_groups<T, 2, 2, SRC>(a, p, st, what);
+  if (a.dqk <= 192 && a.dv <= 128) return launch_groups<T, 3, 2, SRC>(a, p, st, what);
+  return launch_shape<T, 4, 4, 1, SRC>(a, p, st, what);
 }
 
 // Packed rows, and pages of a multiple of 8 rows, are read 8 rows to an instruction through a resource that ends with them
