@@ -25,119 +25,146 @@ struct AppendArgs {
   int q_in_place, k_in_place;  // the dims that do not turn are there already
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendWaves = 4;
 constexpr int kMaxPairs = 128;
 
-// A workgroup takes TPW tokens. Each of its waves finds the streams, positions and page rows of its tokens; then the angles
-// of all pairs are turned into cosines and sines once for all heads; then the items (16 elements of a head that turn, or 8
-// that only move) go through the threads.
-template <class T, int TPW>
-__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
-  __shared__ int s_pos[TPW], s_row[TPW];
-  __shared__ int64_t s_page[TPW];  // -1: the token is not stored
-  __shared__ float s_cos[TPW * kMaxPairs], s_sin[TPW * kMaxPairs];
-  const int tid = threadIdx.x, wave = tid / kWave;
-  const int t0 = static_cast<int>(blockIdx.x) * TPW;
-  for (int j = wave; j < TPW; j += kAppendThreads / kWave) {
-    const int t = t0 + j;
-    int pos = 0, row = 0;
-    int64_t page = -2;  // no stream owns the token: nothing of it is written
-    if (t < a.batch.tokens) {
-      const int b = stream_of_token(a.batch, t);
-      if (b < a.batch.seqs) {
-        const Stream s = stream_at(a.batch, b);
-        page = -1;
-        pos = s.kv < 0 ? 0 : s.kv - s.n + (t - s.first);
-        if (s.kv >= 0 && pos >= 0 && pos < a.batch.max_keys) {
-          const int pg = static_cast<int>(div_by(pos, a.page));
-          const int64_t id = idx_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + pg);
-          row = pos - pg * static_cast<int>(a.page.d);
-          if (id >= 0 && id < a.n_pages) page = id;
-        }
-      }
+// Bound by the bytes: each is read once and written once, with 16-byte accesses of neighbouring lanes (131 MB at 4000 tokens
+// of 16 + 16 heads of 192 and 16 of 128 in 31.8 us: 4.1 TB/s, where a copy of 2 GiB moves 4.9). WPT waves take a token and
+// share its heads; no wave waits for another. A lane keeps one place of a head for all the heads
+// that it goes through: 16 elements that turn, or 8 that only move; its cosines and sines, shared by all heads, come once,
+// from the angles that the wave's lanes turn side by side. The first heads' data, which hang on nothing, are requested
+// before the token's stream, position and page are found.
+template <class T, int WPT>
+__global__ __launch_bounds__(kAppendWaves * kWave) void paged_append_kernel(AppendArgs a) {
+  constexpr int AHEAD = WPT == 1 ? 2 : 3;  // heads of a lane in flight
+  __shared__ __align__(16) float s_cos[kAppendWaves][kMaxPairs], s_sin[kAppendWaves][kMaxPairs];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int t = static_cast<int>(blockIdx.x) * (kAppendWaves / WPT) + wave / WPT, part = wave % WPT;
+  if (t >= a.batch.tokens) return;
+  // the lane's place in a head of q or k
+  const int iph = static_cast<int>(a.iph.d), at_once = kWave / iph, sub = static_cast<int>(div_by(lane, a.iph)), c = lane - sub * iph;
+  const bool turns = c < a.pairs / 8;
+  const int ch = c - a.pairs / 8;
+  const int d0 = !turns ? (ch < a.rot_offset / 8 ? 8 * ch : 8 * ch + 2 * a.pairs) : a.rot_offset + (a.interleaved ? 16 * c : 8 * c);
+  const int d1 = !turns ? d0 : a.interleaved ? d0 + 8 : d0 + a.pairs;
+  const int heads = a.nh + a.nkv, first = part * at_once + sub, step = WPT * at_once;
+  const int last = sub < at_once ? heads : 0;  // lanes behind the last whole head have none
+  const uint16_t *q = a.q.at(t, 0), *k = a.k.at(t, 0), *v = a.v.at(t, 0);
+  auto source = [&](int h) { return h < a.nh ? q + h * a.q.hs : k + (h - a.nh) * a.k.hs; };
+  uint4 x0[AHEAD], x1[AHEAD];
+  auto request = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const uint16_t* s = source(min(h0 + u * step, heads - 1));
+      x0[u] = ld16(s + d0);
+      x1[u] = ld16(s + d1);
     }
-    if (lane_id() == 0) {
-      s_pos[j] = pos;
-      s_row[j] = row;
-      s_page[j] = page;
-    }
+  };
+  request(first);
+  const int vc = a.dv / 8, v_once = kWave / vc, v_sub = lane / vc, vd = 8 * (lane - v_sub * vc);
+  const int v_first = part * v_once + v_sub, v_step = WPT * v_once, v_last = v_sub < v_once ? a.nkv : 0;
+  uint4 xv = ld16(v + min(v_first, a.nkv - 1) * a.v.hs + vd);
+
+  const int b = __builtin_amdgcn_readfirstlane(stream_of_token(a.batch, t));
+  if (b >= a.batch.seqs) return;  // no stream owns the token
+  const Stream s = stream_at(a.batch, b);
+  const int pos = s.kv < 0 ? 0 : s.kv - s.n + (t - s.first);
+  bool stored = s.kv >= 0 && pos >= 0 && pos < a.batch.max_keys;
+  int row = 0;
+  int64_t page = 0;
+  if (stored) {
+    const int pg = static_cast<int>(div_by(pos, a.page));
+    page = value_of(index_at(a.batch.table, a.batch.i64, b * a.batch.table_stride + pg), a.batch.i64);
+    row = pos - pg * static_cast<int>(a.page.d);
+    stored = page >= 0 && page < a.n_pages;
   }
-  __syncthreads();
   // angles in 64 bits, reduced to [-1/2, 1/2] turns: a position of 10^6 leaves 2^-33 of a turn, where 32 bits would leave
   // a hundredth of a turn
-  for (int i = tid; i < TPW * a.pairs; i += kAppendThreads) {
-    const int j = i / a.pairs, p = i - j * a.pairs;
-    const double turns = static_cast<double>(s_pos[j]) * static_cast<double>(a.inv_freq[p]) * 0.15915494309189533577;
-    float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-    s_cos[j * kMaxPairs + p] = c;
-    s_sin[j * kMaxPairs + p] = s;
+  for (int p = lane; p < a.pairs; p += kWave) {
+    const double turn = static_cast<double>(pos) * static_cast<double>(a.inv_freq[p]) * 0.15915494309189533577;
+    float sn, cs;
+    sincospif(2.0f * static_cast<float>(turn - rint(turn)), &sn, &cs);
+    s_cos[wave][p] = cs;
+    s_sin[wave][p] = sn;
   }
-  __syncthreads();
-  const int rot_items = a.pairs / 8, heads = a.nh + a.nkv;
-  const int qk_items = heads * static_cast<int>(a.iph.d), vc = a.dv / 8, items = qk_items + a.nkv * vc;
-  for (int i = tid; i < TPW * items; i += kAppendThreads) {
-    const int j = TPW == 1 ? 0 : i / items, it = i - j * items, t = t0 + j;
-    const int64_t page = s_page[j];
-    if (page == -2) continue;
-    const int row = s_row[j];
-    if (it >= qk_items) {
-      const int h = (it - qk_items) / vc, c = (it - qk_items) - h * vc;
-      if (page >= 0) st16(a.vp.at(page, h, row) + 8 * c, ld16(a.v.at(t, h) + 8 * c));
-      continue;
-    }
-    const int head = static_cast<int>(div_by(it, a.iph)), c = it - head * static_cast<int>(a.iph.d);
-    const bool isq = head < a.nh;
-    const int h = isq ? head : head - a.nh;
-    const uint16_t* src = isq ? a.q.at(t, h) : a.k.at(t, h);
-    uint16_t* dst = isq ? a.q_out.at(t, h) : a.k_out.p ? a.k_out.at(t, h) : nullptr;
-    uint16_t* pool = !isq && page >= 0 ? a.kp.at(page, h, row) : nullptr;
-    if (c >= rot_items) {  // a chunk that does not turn
-      const int ch = c - rot_items, d = ch < a.rot_offset / 8 ? 8 * ch : 8 * ch + 2 * a.pairs;
-      const bool stays = isq ? a.q_in_place : a.k_in_place;
-      if (stays && !pool) continue;
-      const uint4 x = ld16(src + d);
-      if (dst && !stays) st16(dst + d, x);
-      if (pool) st16(pool + d, x);
-      continue;
-    }
-    const int d0 = a.rot_offset + (a.interleaved ? 16 * c : 8 * c), d1 = a.interleaved ? d0 + 8 : d0 + a.pairs;
-    float x0[8], x1[8], y0[8], y1[8];
-    unpack8<T>(ld16(src + d0), x0);
-    unpack8<T>(ld16(src + d1), x1);
-    const float* cs = s_cos + j * kMaxPairs + 8 * c;
-    const float* sn = s_sin + j * kMaxPairs + 8 * c;
-    if (a.interleaved) {
+  wave_lds_fence();
+  float cs[8], sn[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y0[2 * e] = fmaf(x0[2 * e], cs[e], -x0[2 * e + 1] * sn[e]);
-        y0[2 * e + 1] = fmaf(x0[2 * e + 1], cs[e], x0[2 * e] * sn[e]);
-        y1[2 * e] = fmaf(x1[2 * e], cs[4 + e], -x1[2 * e + 1] * sn[4 + e]);
-        y1[2 * e + 1] = fmaf(x1[2 * e + 1], cs[4 + e], x1[2 * e] * sn[4 + e]);
-      }
-    } else {
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = turns ? s_cos[wave][8 * c + e] : 1.f;
+    sn[e] = turns ? s_sin[wave][8 * c + e] : 0.f;
+  }
+  uint16_t* q_out = a.q_out.at(t, 0);
+  uint16_t* k_out = a.k_out.p ? a.k_out.at(t, 0) : nullptr;
+  uint16_t* k_row = a.kp.at(stored ? page : 0, 0, row);
+  for (int h0 = first; h0 < last; h0 += AHEAD * step) {
+    if (h0 != first) request(h0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y0[e] = fmaf(x0[e], cs[e], -x1[e] * sn[e]);
-        y1[e] = fmaf(x1[e], cs[e], x0[e] * sn[e]);
+    for (int u = 0; u < AHEAD; ++u) {
+      const int h = h0 + u * step;
+      if (h >= last) break;
+      const bool isq = h < a.nh;
+      uint16_t* dst = isq ? q_out + h * a.q_out.hs : k_out ? k_out + (h - a.nh) * a.k_out.hs : nullptr;
+      uint16_t* pool = !isq && stored ? k_row + (h - a.nh) * a.kp.hs : nullptr;
+      uint4 w0 = x0[u], w1 = x1[u];
+      if (turns) {
+        float a0[8], a1[8], y0[8], y1[8];
+        unpack8<T>(w0, a0);
+        unpack8<T>(w1, a1);
+        if (a.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y0[2 * e] = fmaf(a0[2 * e], cs[e], -a0[2 * e + 1] * sn[e]);
+            y0[2 * e + 1] = fmaf(a0[2 * e + 1], cs[e], a0[2 * e] * sn[e]);
+            y1[2 * e] = fmaf(a1[2 * e], cs[4 + e], -a1[2 * e + 1] * sn[4 + e]);
+            y1[2 * e + 1] = fmaf(a1[2 * e + 1], cs[4 + e], a1[2 * e] * sn[4 + e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            y0[e] = fmaf(a0[e], cs[e], -a1[e] * sn[e]);
+            y1[e] = fmaf(a1[e], cs[e], a0[e] * sn[e]);
+          }
+        }
+        w0 = pack8<T>(y0);
+        w1 = pack8<T>(y1);
+      } else if (isq ? a.q_in_place : a.k_in_place) {
+        dst = nullptr;
+      }
+      if (dst) {
+        st16(dst + d0, w0);
+        if (turns) st16(dst + d1, w1);
+      }
+      if (pool) {
+        st16(pool + d0, w0);
+        if (turns) st16(pool + d1, w1);
       }
     }
-    const uint4 w0 = pack8<T>(y0), w1 = pack8<T>(y1);
-    if (dst) {
-      st16(dst + d0, w0);
-      st16(dst + d1, w1);
-    }
-    if (pool) {
-      st16(pool + d0, w0);
-      st16(pool + d1, w1);
-    }
+  }
+  if (!stored) return;
+  uint16_t* v_row = a.vp.at(page, 0, row);
+  for (int h = v_first; h < v_last; h += v_step) {
+    st16(v_row + h * a.vp.hs + vd, xv);
+    xv = ld16(v + min(h + v_step, a.nkv - 1) * a.v.hs + vd);
   }
 }
 
+template <class T, int WPT>
+int launch_append(const AppendArgs& a, hipStream_t st) {
+  constexpr int PER = kAppendWaves / WPT;  // tokens of a workgroup
+  hipLaunchKernelGGL((paged_append_kernel<T, WPT>), dim3(static_cast<unsigned>((a.batch.tokens + PER - 1) / PER)),
+                     dim3(kAppendWaves * kWave), 0, st, a);
+  return mm::check_launch("paged_append");
+}
+
+// One wave to a token, or four where the tokens alone leave the device idle and a token is more than a wave's one round. us
+// a call, one wave | four (heads q/k: tokens): 16/16 of 192: 500 tokens 12.9 | 7.8, 4000 31.8 | 34.0; 32/8 of 128: 128 tokens
+// 6.8 | 5.4, 2000 12.4 | 14.8; 14/2 of 64: 64 tokens 4.8 | 4.8, 2549 6.5 | 12.0, 20000 23.4 | 68.0 (a token a workgroup
+// before that, whose threads all waited for its position: 37.7 at 4000 tokens, 61.6 at 20000).
 template <class T>
 int launch_append(const AppendArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((paged_append_kernel<T, 1>), dim3(static_cast<unsigned>(a.batch.tokens)), dim3(kAppendThreads), 0, st, a);
-  return mm::check_launch("paged_append");
+  const int64_t items = (a.nh + a.nkv) * static_cast<int64_t>(a.iph.d);
+  return a.batch.tokens < 4 * mm::cu_count() && items > 2 * kWave ? launch_append<T, 4>(a, st) : launch_append<T, 1>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------ checks on the host
