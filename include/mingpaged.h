@@ -74,8 +74,10 @@ int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, in
                     const float* inv_freq, int64_t pairs, int rot_offset, int interleaved, void* q_out, int64_t qo_ts,
                     int64_t qo_hs, void* k_out, int64_t ko_ts, int64_t ko_hs, void* stream);
 
-/* Bytes of workspace mm_paged_attn needs for a batch of these sizes (max_keys = max_pages * page); -1 if invalid. */
-int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+/* Bytes of workspace mm_paged_attn needs for a batch of these sizes (max_keys = max_pages * page), or with at_most != 0
+ * for every batch of at most these tokens, streams and keys; 0: none, -1 if invalid. */
+int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv,
+                                int at_most);
 
 /* Attention of the new tokens over the paged cache that already holds their own rows (mm_paged_append): token i of stream
  * b, at position p = kv_lens[b] - n_b + i, takes softmax(scale * q . K[0..p]^T) . V[0..p], query head h on key / value
@@ -83,14 +85,16 @@ int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, 
  * aligned, of out 8-byte). Scores, statistics and sums in fp32; the weights enter the value product rounded to the cache's
  * type. Positions whose page id lies outside [0, n_pages) are left out; a token with no position left gets zeros; the
  * tokens of a stream whose kv_lens lies outside [0, max_pages * page] get NaN. Rows past a token's position never reach
- * it, whatever they hold. out must not overlap q or the pool. workspace: mm_paged_attn_workspace bytes, 16-byte aligned,
- * no initialisation; calls that share one must not overlap in time. */
+ * it, whatever they hold. out must not overlap q or the pool. workspace: mm_paged_attn_workspace bytes, 16-byte aligned
+ * (NULL where that is 0), no initialisation; calls that share one must not overlap in time. Equal calls give equal bits; the
+ * order of a token's sums depends on the whole batch's lengths. Limits: tokens 2^22, tokens * nh 2^30, streams 2^20,
+ * max_pages * page 2^30. */
 int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
                   float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace, int64_t workspace_bytes,
                   void* stream);
 
-/* Bytes of workspace mm_prompt_attn needs; -1 if invalid. */
-int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv);
+/* Bytes of workspace mm_prompt_attn needs, as mm_paged_attn_workspace. */
+int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv, int at_most);
 
 /* Causal attention over whole prompts packed one behind the other: token i of prompt b (tokens cu[b] .. cu[b+1] - 1)
  * takes softmax(scale * q . K[0..i]^T) . V[0..i] over its own prompt's rows of k [tokens, nkv, dqk] and v [tokens, nkv,

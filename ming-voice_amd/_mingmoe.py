@@ -123,10 +123,10 @@ PAGED_VERSION = 1
 PAGED_SIGNATURES = {
     "mm_paged_version": ([], ctypes.c_int),
     "mm_paged_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P], ctypes.c_int),
-    "mm_paged_attn_workspace": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
+    "mm_paged_attn_workspace": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32], _I64),
     "mm_paged_attn": ([_P, _I64, _I64, _I32, _P, _P, _F32, _P, _I64, _I64, _P,
                        _I64, _P], ctypes.c_int),
-    "mm_prompt_attn_workspace": ([_I64, _I64, _I32, _I32, _I32, _I32], _I64),
+    "mm_prompt_attn_workspace": ([_I64, _I64, _I32, _I32, _I32, _I32, _I32], _I64),
     "mm_prompt_attn": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64,
                         _I64, _F32, _P, _I64, _I64, _P, _I64, _P], ctypes.c_int),
 }

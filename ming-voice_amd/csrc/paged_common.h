@@ -219,7 +219,7 @@ __device__ __forceinline__ int cut_of(const AttnArgs& a, const Stream& mine, Loa
   }
   // rounded up by more than the sum over the lanes can lose, so that no cut gives more pieces than target
   const float cut = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / static_cast<float>(a.target));
-  return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), 1073741824.f));
+  return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), static_cast<float>((1 << 30) / GR)));
 }
 
 // The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the batch itself: streams 64 at a
@@ -428,8 +428,8 @@ struct AttnPlan {
   int64_t blocks, target, workspace;
 };
 AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
-// The most workspace that a call of at most these tokens, streams and keys takes.
-int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv);
+// Its workspace, or with at_most the most that any call of at most these tokens, streams and keys takes.
+int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv, bool at_most);
 int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
 int launch_many(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what);
 int launch_join_many(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st, const char* what);

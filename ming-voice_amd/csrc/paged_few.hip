@@ -453,25 +453,61 @@ int launch_type(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char
 
 }  // namespace
 
+namespace {
+
+int64_t most_blocks(int64_t rows, int64_t seqs, int64_t br) { return rows / br + seqs < rows ? rows / br + seqs : rows; }
+
+// Bytes of keys and values that blocks of 16 rows would read, each all the keys that its stream can have.
+int64_t reads_of_few(int64_t rows, int64_t seqs, int64_t max_keys, int nkv, int dqk, int dv) {
+  return most_blocks(rows, seqs, 16) * nkv * (dqk + dv) * 2 * max_keys;
+}
+constexpr int64_t kFewReads = 64 << 20;
+
+int64_t few_granule(int dqk, int dv) { return (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys; }
+// pieces aimed at for one key / value head
+int64_t few_target(int nkv) { return (4 * mm::cu_count() + nkv - 1) / nkv; }
+int64_t many_target(int nkv) { return (2 * mm::cu_count() + nkv - 1) / nkv; }
+int64_t state_bytes(int64_t target, int nkv, int br, int dv) { return 2 * target * nkv * br * (dv + 2) * 4; }
+
+}  // namespace
+
+// Few rows or many: 16-row blocks where the streams have no more rows than that on average (a decode step), and where the
+// keys that such blocks read are so few that the caches bring them quicker than 128 rows get through them. us a call, 16 |
+// 128 rows (reads at 16): a prompt of 37 Talker tokens 5.0 | 6.2, of 200 5.6 | 9.2 (9 MB), of 500 8.0 | 13.2 (56 MB); 100
+// Talker tokens behind 1000 13.6 | 15.6 (25 MB); 20 heads of one key / value head behind 6000 10.7 | 16.6 (3 MB); 30 thinker
+// tokens behind 3000 23.9 | 23.2 (62 MB); 300 tokens of 32/8 heads of 128 16.9 | 13.7 (92 MB); 64 tokens of those behind 8000
+// 66 | 39 (528 MB).
+// Cutting: few rows above 4 granules of keys (one stream at 700 positions: 10.0 us cut, 8.4 not), then 4 pieces a CU (decode of
+// 16 streams behind 4000 to 40000 positions: 397 us uncut, 239 at 1 piece a CU, 217 at 2, 206 at 4, 202 at 8). Many rows over
+// a cache: 2 pieces a CU of at least 4 granules (pieces of 100 to 500 tokens behind 611 to 5000 positions: 149 us uncut, 98
+// at 1, 91 at 2, 101 at 3, 103 at 4; 512 tokens behind 30000: 798 uncut, 414, 316, 386 at 2.5). Prompts, whose keys are
+// their own tokens, only where their row blocks leave half of the CUs idle (12 ragged Talker prompts: 42 us uncut, 47 cut).
+// Two groups of waves to a block where a prompt's blocks are fewer than 4 a CU: they halve the time of the last block (12
+// ragged Talker prompts 42.8 -> 38.5 us, 2000 Talker tokens 37.4 -> 29.6, 4000 72 -> 59), but in a long run two workgroups
+// of one group mix matrix and vector work better (8192 tokens of 32/8 heads of 128: 590 | 643), and over a cache the cut
+// does as much (91 | 95).
 AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
   AttnPlan p{};
   const int64_t rows = tokens * (nh / nkv), cus = mm::cu_count();
-  auto blocks_of = [&](int64_t br) { return rows / br + seqs < rows ? rows / br + seqs : rows; };
-  const int64_t reads = blocks_of(16) * nkv * max_keys * (dqk + dv) * 2;
-  p.many = rows > 16 * seqs && reads > (64LL << 20);
-  p.blocks = blocks_of(p.many ? 128 : 16);
+  p.many = rows > 16 * seqs && reads_of_few(rows, seqs, max_keys, nkv, dqk, dv) > kFewReads;
+  p.blocks = most_blocks(rows, seqs, p.many ? 128 : 16);
   if (p.many) {
-    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus) p.target = (2 * cus + nkv - 1) / nkv;
-    p.groups = !paged && p.target == 0 && p.blocks * nkv < 4 * cus ? 2 : 1;
-  } else if (max_keys > 4 * (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys) {
-    p.target = (4 * cus + nkv - 1) / nkv;
+    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus) p.target = many_target(nkv);
+    p.groups = !paged && p.target == 0 && p.blocks * nkv < 4 * cus && dqk <= 192 && dv <= 128 ? 2 : 1;
+    p.workspace = state_bytes(p.target, nkv, 128, dv);
+  } else {
+    if (max_keys > 4 * few_granule(dqk, dv)) p.target = few_target(nkv);
+    p.workspace = state_bytes(p.target, nkv, 16, dv);
   }
-  p.workspace = 2 * p.target * nkv * (p.many ? 128 : 16) * (dv + 2) * 4;
   return p;
 }
 
-int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
-  return plan_attn(paged, tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
+int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv, bool at_most) {
+  if (!at_most) return plan_attn(paged, tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
+  const int64_t few = max_keys > 4 * few_granule(dqk, dv) ? state_bytes(few_target(nkv), nkv, 16, dv) : 0;
+  const bool many = max_keys > 64 * kMinCut && reads_of_few(tokens * (nh / nkv), seqs, max_keys, nkv, dqk, dv) > kFewReads;
+  const int64_t of_many = many ? state_bytes(many_target(nkv), nkv, 128, dv) : 0;
+  return few > of_many ? few : of_many;
 }
 
 int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {

@@ -68,6 +68,7 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void paged_append_kernel(Appe
   const int b = __builtin_amdgcn_readfirstlane(stream_of_token(a.batch, t));
   if (b >= a.batch.seqs) return;  // no stream owns the token
   const Stream s = stream_at(a.batch, b);
+  if (t < s.first || t >= s.first + s.n) return;
   const int pos = s.kv < 0 ? 0 : s.kv - s.n + (t - s.first);
   bool stored = s.kv >= 0 && pos >= 0 && pos < a.batch.max_keys;
   int row = 0;
@@ -169,7 +170,9 @@ int launch_append(const AppendArgs& a, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------ checks on the host
 
-constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxKeys = (1LL << 31) - 1;
+constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxPages = (1LL << 31) - 1;
+// positions of a stream, and rows (tokens times heads): 32-bit numbers of them stay positive with a tile or a piece added
+constexpr int64_t kMaxKeys = 1LL << 30, kMaxRows = 1LL << 30;
 
 // A row of strides; those of a dim of one are not used and may be anything.
 int check_rows(const char* what, const char* name, const void* p, int64_t tokens, int64_t ts, int heads, int64_t hs, int align) {
@@ -202,10 +205,10 @@ int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) 
   if (rc) return rc;
   if ((rc = check_tokens(what, b->tokens, b->seqs))) return rc;
   MM_REQUIRE(b->idx_dtype == MM_INT32 || b->idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
-  MM_REQUIRE(b->tokens * nh <= kMaxKeys, "%s: tokens * nh must be below 2^31", what);
-  MM_REQUIRE(g->page >= 1 && g->n_pages >= 0 && g->n_pages <= kMaxKeys && b->max_pages >= 0 && b->table_stride >= 0, "%s: bad page or table sizes", what);
-  MM_REQUIRE(b->max_pages <= kMaxKeys / g->page, "%s: max_pages * page must be below 2^31", what);
-  MM_REQUIRE(b->cu && b->kv_lens && (b->table || b->max_pages == 0), "%s: null batch array", what);
+  MM_REQUIRE(b->tokens * nh <= kMaxRows, "%s: tokens * nh must be at most 2^30", what);
+  MM_REQUIRE(g->page >= 1 && g->n_pages >= 0 && g->n_pages <= kMaxPages && b->max_pages >= 0 && b->table_stride >= 0, "%s: bad page or table sizes", what);
+  MM_REQUIRE(b->max_pages <= kMaxKeys / g->page, "%s: max_pages * page must be at most 2^30", what);
+  MM_REQUIRE(b->seqs == 0 || (b->cu && b->kv_lens && (b->table || b->max_pages == 0)), "%s: null batch array", what);
   MM_REQUIRE(g->n_pages == 0 || (g->k && g->v), "%s: null pool", what);
   MM_REQUIRE(mm::aligned16(g->k) && mm::aligned16(g->v), "%s: the pool must be 16-byte aligned", what);
   const int64_t st[6] = {g->k_page_stride, g->k_head_stride, g->k_row_stride, g->v_page_stride, g->v_head_stride, g->v_row_stride};
@@ -234,7 +237,7 @@ int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int
   a.scale = scale == 0.f ? 1e-37f : fabsf(scale);
   a.negative = scale < 0.f;
   const AttnPlan p = plan_attn(paged, a.batch.tokens, a.batch.seqs, max_keys, a.nh, a.nkv, a.dqk, a.dv);
-  MM_REQUIRE((p.blocks + p.target) * a.nkv <= 0x7fffffff, "%s: too many rows", what);
+  MM_REQUIRE((p.blocks + p.target) * a.nkv < (1LL << 23), "%s: too many streams and rows for one launch", what);
   MM_REQUIRE(p.workspace == 0 || (workspace && mm::aligned16(workspace) && workspace_bytes >= p.workspace),
              "%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)p.workspace);
   a.ws = static_cast<float*>(workspace);
@@ -291,11 +294,14 @@ extern "C" int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const 
   return pages->dtype == MM_BF16 ? launch_append<BF16>(a, MM_STREAM(stream)) : launch_append<FP16>(a, MM_STREAM(stream));
 }
 
-extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv) {
-  if (check_shape("paged_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("paged_attn", tokens, seqs) || max_keys < 0 ||
-      max_keys > kMaxKeys)
+extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv,
+                                           int at_most) {
+  if (check_shape("paged_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("paged_attn", tokens, seqs)) return -1;
+  if (max_keys < 0 || max_keys > kMaxKeys) {
+    mm::set_error(MM_ERR_ARG, "paged_attn: bad max_keys=%lld", (long long)max_keys);
     return -1;
-  return workspace_of(true, tokens, seqs, max_keys, nh, nkv, dqk, dv);
+  }
+  return workspace_of(true, tokens, seqs, max_keys, nh, nkv, dqk, dv, at_most != 0);
 }
 
 extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
@@ -322,9 +328,9 @@ extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, 
   return attend(a, pages->dtype, true, scale, workspace, workspace_bytes, MM_STREAM(stream), what);
 }
 
-extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv) {
+extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv, int at_most) {
   if (check_shape("prompt_attn", MM_BF16, nh, nkv, dqk, dv) || check_tokens("prompt_attn", tokens, seqs)) return -1;
-  return workspace_of(false, tokens, seqs, tokens, nh, nkv, dqk, dv);
+  return workspace_of(false, tokens, seqs, tokens, nh, nkv, dqk, dv, at_most != 0);
 }
 
 extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
@@ -336,8 +342,8 @@ extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const v
   if (rc) return rc;
   if ((rc = check_tokens(what, tokens, seqs))) return rc;
   MM_REQUIRE(idx_dtype == MM_INT32 || idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
-  MM_REQUIRE(cu, "%s: null cu", what);
-  MM_REQUIRE(tokens * nh <= kMaxKeys, "%s: tokens * nh must be below 2^31", what);
+  MM_REQUIRE(cu || seqs == 0, "%s: null cu", what);
+  MM_REQUIRE(tokens * nh <= kMaxRows, "%s: tokens * nh must be at most 2^30", what);
   if (tokens == 0 || seqs == 0) return MM_OK;
   if ((rc = check_rows(what, "q", q, tokens, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "k", k, tokens, k_ts, nkv, k_hs, 16)) ||
       (rc = check_rows(what, "v", v, tokens, v_ts, nkv, v_hs, 16)) || (rc = check_rows(what, "out", out, tokens, o_ts, nh, o_hs, 8)))

@@ -447,6 +447,37 @@ def test_two_streams_at_once():
 def test_a_small_workspace_is_refused():
     s = Streams([1], [9000], seed=79)
     ws = PK.paged_attn_workspace(1, 1, s.table.shape[1] * s.page, s.nh, s.nkv, s.dqk, s.dv)
-    if ws.numel() > 16:
-        with pytest.raises(ValueError, match="workspace"):
-            s.attn(workspace=ws[:-16])
+    assert torch.equal(s.attn(workspace=ws), s.attn())
+    with pytest.raises(ValueError, match="workspace"):
+        s.attn(workspace=ws[:-16])
+    with pytest.raises(ValueError, match="dv=12"):
+        PK.prompt_attn_workspace(8, 2, 4, 2, 64, 12)
+
+
+def test_no_streams_no_tokens_no_pages():
+    e = torch.empty(0, device=DEV, dtype=torch.int32)
+    cu = torch.zeros(1, device=DEV, dtype=torch.int32)
+    q, k = torch.full((3, 4, 64), 2.0, device=DEV, dtype=BF), torch.zeros(3, 2, 64, device=DEV, dtype=BF)
+    pool = torch.zeros(0, 2, 16, 64, device=DEV, dtype=BF)
+    out = torch.full_like(q, 7.0)
+    assert (PK.paged_attn(q, pool, pool, e.view(0, 5), cu, e, out=out) == 7.0).all()
+    assert (PK.prompt_attn(q, k, k, cu, out=out) == 7.0).all()
+    assert (PK.paged_append(q, k, k, pool, pool, e.view(0, 5), cu, e, q_out=out) == 7.0).all()
+    one = torch.tensor([0, 3], device=DEV, dtype=torch.int32)
+    zero = torch.zeros(1, device=DEV, dtype=torch.int32)
+    assert (PK.paged_attn(q, pool, pool, zero.view(1, 1)[:, :0], one, zero, out=out) == 0.0).all()  # nothing to see
+    assert torch.equal(PK.paged_append(q, k, k, pool, pool, zero.view(1, 1)[:, :0], one, zero), q)
+    none = PK.paged_attn(q[:0], pool, pool, zero.view(1, 1), zero.expand(2).contiguous(), zero)
+    assert none.shape == (0, 4, 64)
+
+
+def test_indices_that_make_no_sense_stay_in_bounds():
+    """cu_seqlens that falls, starts behind 0 or ends behind the tokens: which rows are computed is open, but every access
+    stays inside the tensors (the host-side twin of the work's division: tests/test_paged_kv.py)."""
+    s = Streams([5, 60, 3], [100, 900, 0], seed=83)
+    for cu in ([0, 65, 5, 68], [3, 5, 65, 68], [0, 5, 65, 9999], [-7, 5, 65, 68], [68, 0, 68, 0], [0, 68, 0, 68]):
+        s.cu = torch.tensor(cu, device=DEV, dtype=torch.int32)
+        s.attn()
+        PK.prompt_attn(s.q, s.k, s.v, s.cu)
+        PK.paged_append(s.q, s.k, s.v, s.kp, s.vp, s.table, s.cu, s.lens)
+        torch.cuda.synchronize()

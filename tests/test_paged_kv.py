@@ -31,7 +31,7 @@ def test_header_declares_the_entry_points_and_the_library_exports_them():
 
 
 # digests of the header's interface (no comments) by version, as tests/test_abi.py keeps them for mingmoe.h
-INTERFACES = {1: "d5929419b43b0513"}
+INTERFACES = {1: "4173de86697e9f74"}
 
 
 def test_the_version_moves_with_the_interface():
@@ -99,7 +99,7 @@ def prompt(q=P, k=P, v=P, dtype=mm.MM_BF16, nh=14, nkv=2, dqk=64, dv=64, cu=P, i
     ("bf16 or fp16", dict(dtype=mm.MM_FP32), {}), ("multiple of nkv", dict(nkv=4), {}), ("multiple of nkv", dict(nkv=0), {}),
     ("dqk=60", dict(dqk=60), {}), ("dqk=264", dict(dqk=264), {}), ("dv=0", dict(dv=0), {}), ("dv=260", dict(dv=260), {}),
     ("page or table", dict(page=0), {}), ("page or table", dict(n_pages=-1), {}), ("page or table", {}, dict(max_pages=-1)),
-    ("below 2^31", dict(page=1 << 20), dict(max_pages=1 << 11)), ("tokens -1", {}, dict(tokens=-1)),
+    ("at most 2^30", dict(page=1 << 20), dict(max_pages=1 << 11)), ("tokens -1", {}, dict(tokens=-1)),
     ("tokens", {}, dict(tokens=1 << 23)), ("streams", {}, dict(seqs=-1)), ("streams", {}, dict(seqs=1 << 21)),
     ("int32 or int64", {}, dict(idx_dtype=mm.MM_FP32)), ("null batch", {}, dict(cu=None)),
     ("null batch", {}, dict(kv_lens=None)), ("null batch", {}, dict(table=None)), ("null pool", dict(v=None), {}),
@@ -125,7 +125,7 @@ def test_attn_refuses():
     assert "strides of q" in err(attn(q_ts=892)) and "out must be 8-byte" in err(attn(out=P + 4))
     assert "strides of out" in err(attn(o_hs=66))
     assert "tokens * nh" in err(attn(b=batch(tokens=1 << 22), nh=512))
-    need = mm.load().mm_paged_attn_workspace(5, 3, 16 * 1000, 14, 2, 64, 64)  # a table that allows long contexts
+    need = mm.load().mm_paged_attn_workspace(5, 3, 16 * 1000, 14, 2, 64, 64, 0)  # a table that allows long contexts
     long = batch(max_pages=1000, table_stride=1000)
     assert need > 0 and "workspace" in err(attn(b=long, ws_bytes=need - 1)) and "workspace" in err(attn(b=long, ws=None))
     assert "workspace" in err(attn(b=long, ws=P + 4))
@@ -145,15 +145,41 @@ def test_nothing_to_do_is_done_without_a_gpu():
     assert prompt(tokens=0) == 0 and prompt(seqs=0) == 0
 
 
-def test_workspace_sizes_are_refused_or_bounded():
+def test_no_streams_need_no_arrays():
+    assert attn(b=batch(seqs=0, cu=None, kv_lens=None, table=None)) == 0
+    assert append(b=batch(seqs=0, cu=None, kv_lens=None, table=None)) == 0 and prompt(seqs=0, cu=None) == 0
+
+
+def test_more_than_one_launch_holds_is_refused():
+    g, b = pages(nkv=16, k_head_stride=64, v_head_stride=64), batch(seqs=1 << 20, tokens=1 << 22)
+    assert "one launch" in err(attn(g=g, b=b, nh=64))
+
+
+def test_workspace_sizes():
     lib = mm.load()
-    assert lib.mm_paged_attn_workspace(-1, 1, 64, 14, 2, 64, 64) == -1
-    assert lib.mm_paged_attn_workspace(1, 1, 1 << 31, 14, 2, 64, 64) == -1
-    assert lib.mm_paged_attn_workspace(1, 1, 64, 14, 4, 64, 64) == -1
-    assert lib.mm_prompt_attn_workspace(1, -1, 14, 2, 64, 64) == -1 and lib.mm_prompt_attn_workspace(1, 1, 14, 2, 64, 63) == -1
-    with pytest.raises(ValueError, match="dv=12"):
-        PK.prompt_attn_workspace(8, 2, 4, 2, 64, 12, device="cpu")
-    assert PK.paged_attn_workspace(1, 1, 64, 14, 2, 64, 64, device="cpu").numel() >= 16
+    assert lib.mm_paged_attn_workspace(-1, 1, 64, 14, 2, 64, 64, 0) == -1
+    assert lib.mm_paged_attn_workspace(1, 1, 1 << 31, 14, 2, 64, 64, 1) == -1
+    assert lib.mm_paged_attn_workspace(1, 1, 64, 14, 4, 64, 64, 0) == -1
+    assert lib.mm_prompt_attn_workspace(1, -1, 14, 2, 64, 64, 0) == -1
+    assert lib.mm_prompt_attn_workspace(1, 1, 14, 2, 64, 63, 1) == -1
+    assert lib.mm_paged_attn_workspace(1, 1, 700, 14, 2, 64, 64, 0) == 0  # a short table is not cut
+
+
+@pytest.mark.parametrize("nh,nkv,dqk,dv", [(14, 2, 64, 64), (16, 16, 192, 128), (32, 8, 128, 128), (16, 2, 256, 256),
+                                           (20, 1, 64, 64)])
+def test_a_workspace_for_at_most_these_sizes_serves_every_smaller_batch(nh, nkv, dqk, dv):
+    lib = mm.load()
+    sizes = [1, 2, 15, 64, 130, 700, 2500, 9000, 40000]
+    for tokens in sizes:
+        for seqs in (1, 3, 40, 600):
+            most = lib.mm_prompt_attn_workspace(tokens, seqs, nh, nkv, dqk, dv, 1)
+            assert all(lib.mm_prompt_attn_workspace(t, s, nh, nkv, dqk, dv, 0) <= most
+                       for t in sizes if t <= tokens for s in (1, 2, 3, 39, 40, 600) if s <= seqs)
+            for keys in (64, 300, 2000, 50000):
+                most = lib.mm_paged_attn_workspace(tokens, seqs, keys, nh, nkv, dqk, dv, 1)
+                assert all(lib.mm_paged_attn_workspace(t, s, k, nh, nkv, dqk, dv, 0) <= most
+                           for t in sizes if t <= tokens for s in (1, 2, 40, 600) if s <= seqs
+                           for k in (64, 299, 300, 1100, 2000, 50000) if k <= keys)
 
 
 # ------------------------------------------------------------------------------------------------ refusals, wrappers
@@ -263,3 +289,113 @@ def test_oracle_matches_torch_attention():
     got, _, _ = O.paged_attn(part, pool_k, pool_v, table, torch.tensor([0, 2, 2, 4]), torch.tensor([3, 0, 4]), 0.3)
     assert (got[0] == 0).all()  # its only positions lie in the missing page
     torch.testing.assert_close(got[1], v[2].repeat_interleave(2, 0))
+
+
+# ------------------------------------------------------------------------------------------------ the division of the work
+
+class Division:
+    """The kernels' division of an attention's work (csrc/paged_common.h: stream_at, cut_of, find_work, keys_of, pieces_of),
+    number by number, for blocks of `br` rows and granules of `gr` keys."""
+
+    def __init__(self, cu, lens, tokens, group, max_keys, br, gr, target, min_cut):
+        self.br, self.gr, self.group, self.target = br, gr, group, target
+        self.streams = []
+        for c0, c1, kv in zip(cu, cu[1:], lens):
+            first = min(max(c0, 0), tokens)
+            self.streams.append((first, min(max(c1, first), tokens) - first, kv if 0 <= kv <= max_keys else -1))
+        total = sum(self.blocks(s) * -(-max(s[2], 0) // gr) for s in self.streams)
+        self.cut = 0
+        if target:
+            # the kernel's sum over the lanes is in fp32, rounded up by 1e-5 of it: the least and the most that it can be
+            self.cut = min(max(-(-int(total * 1.00002) // target), min_cut), (1 << 30) // gr)
+            assert self.cut * target >= total or self.cut == (1 << 30) // gr
+
+    def blocks(self, s):
+        return -(-s[1] * self.group // self.br)
+
+    def pieces(self, keys):
+        return 1 if self.cut == 0 else max(1, -(--(-keys // self.gr) // self.cut))
+
+    def keys(self, s, blk):
+        last = min(blk * self.br + self.br, s[1] * self.group) - 1
+        return 0 if s[2] < 0 else max(0, s[2] - s[1] + last // self.group + 1)
+
+    def find(self, w, cut_blocks=False):
+        """(stream, block, piece, first slot) of workgroup w, or None."""
+        slots = 0
+        for b, s in enumerate(self.streams):
+            nb, p = self.blocks(s), self.pieces(max(s[2], 0))
+            held = nb * p if p > 1 else 0
+            units = (nb if held else 0) if cut_blocks else nb * p
+            if w < units:
+                at = w if cut_blocks else w // p
+                slot = slots + at * p
+                if w < 0 or at >= nb or (p > 1 and not 0 <= slot <= 2 * self.target - p):
+                    return None
+                return b, nb - 1 - at, 0 if cut_blocks else w - at * p, slot
+            w -= units
+            slots += held
+        return None
+
+
+def _divisions(seed):
+    import random
+    r = random.Random(seed)
+    for _ in range(8):
+        n = r.choice([1, 2, 5, 64, 65, 200])
+        new = [r.choice([0, 1, 1, 1, 3, 40, 700]) for _ in range(n)]
+        lens = [m + r.choice([0, 0, 5, 900, 30000]) for m in new]
+        br, gr, cut = r.choice([(16, 256, 1), (16, 128, 1), (128, 64, 4)])
+        yield new, lens, r.choice([1, 2, 7, 20]), br, gr, cut, r.choice([1, 7, 64, 256])
+
+
+@pytest.mark.parametrize("seed", range(5))
+def test_the_work_is_divided_once_and_within_its_bounds(seed):
+    for new, lens, group, br, gr, min_cut, target in _divisions(seed):
+        cu = [sum(new[:i]) for i in range(len(new) + 1)]
+        N, most = cu[-1], max(lens) + 1
+        d = Division(cu, lens, N, group, most, br, gr, target, min_cut)
+        rows = N * group
+        blocks = min(rows // br + len(new), rows)
+        grid = blocks + target  # what the host launches for these sizes
+        done, slots = set(), {}
+        for w in range(grid):
+            f = d.find(w)
+            if f is None:
+                continue
+            b, blk, piece, slot = f
+            s = d.streams[b]
+            pieces = d.pieces(d.keys(s, blk))
+            if piece >= pieces:
+                continue
+            assert (b, blk, piece) not in done
+            done.add((b, blk, piece))
+            if pieces > 1:
+                assert 0 <= slot + piece < 2 * target and slots.setdefault(slot + piece, (b, blk, piece)) == (b, blk, piece)
+                assert piece * d.cut * gr < d.keys(s, blk)
+        want = {(b, blk, p) for b, s in enumerate(d.streams) for blk in range(d.blocks(s)) for p in range(d.pieces(d.keys(s, blk)))}
+        assert done == want
+        cut = {(b, blk) for b, blk, p in want if p}
+        joined = [d.find(w, cut_blocks=True) for w in range(min(blocks, target))]
+        joined = {f[:2]: f[3] for f in joined if f and d.pieces(d.keys(d.streams[f[0]], f[1])) > 1}
+        assert set(joined) == cut and all(slots[joined[c]] == (*c, 0) for c in cut)
+
+
+@pytest.mark.parametrize("cu", [[0, 65, 5, 68], [3, 5, 65, 68], [0, 5, 65, 9999], [-7, 5, 65, 68], [68, 0, 68, 0],
+                                [0, 68, 0, 68], [1 << 40, -(1 << 40), 1 << 62, 0]])
+@pytest.mark.parametrize("br,gr,min_cut,target", [(16, 256, 1, 0), (16, 256, 1, 5), (128, 64, 4, 3)])
+def test_a_division_of_nonsense_stays_in_bounds(cu, br, gr, min_cut, target):
+    N, group, lens, most = 68, 7, [105, 960, 3], 970
+    d = Division(cu, lens, N, group, most, br, gr, target, min_cut)
+    for w in range(min(N * group // br + 3, N * group) + target):
+        for cut_blocks in (False, True):
+            f = d.find(w, cut_blocks)
+            if f is None:
+                continue
+            b, blk, piece, slot = f
+            first, n, kv = d.streams[b]
+            assert 0 <= blk < d.blocks(d.streams[b]) and 0 <= first and first + n <= N
+            last = min(blk * br + br, n * group) - 1
+            assert 0 <= last // group < n and d.keys(d.streams[b], blk) <= kv <= most
+            if d.pieces(max(kv, 0)) > 1:
+                assert 0 <= slot and slot + d.pieces(max(kv, 0)) <= 2 * target
