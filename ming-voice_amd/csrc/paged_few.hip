@@ -8,10 +8,10 @@ namespace {
 
 constexpr int kKeys = 32;  // keys per tile
 
-// The shape of few_kernel: QF 16-row fragments, NW waves, head dims up to 32 NKQ (q, k) and 16 NT (v).
-template <int QF, int NW, int NKQ, int NT>
+// The shape of few_kernel: NW waves, head dims up to 32 NKQ (q, k) and 16 NT (v).
+template <int NW, int NKQ, int NT>
 struct Few {
-  static constexpr int BR = 16 * QF;
+  static constexpr int BR = 16;
   static constexpr int GR = NW * kKeys;                  // a granule: a tile for every wave
   static constexpr int DVM = 16 * NT;
   static constexpr int KC = 4 * NKQ, VC = 2 * NT;        // 16-byte chunks of a key, value row in LDS
@@ -26,7 +26,7 @@ struct Few {
   static_assert(LDS <= 160 * 1024 && KI % 2 == 0 && NT % 4 == 0, "tile shape");
 };
 
-// Softmax attention of up to 16 QF rows over a piece of their keys, one pass with a running maximum and sum. Grid (work x key /
+// Softmax attention of up to 16 rows over a piece of their keys, one pass with a running maximum and sum. Grid (work x key /
 // value heads) x NW waves. Wave w takes tiles w, w + NW, ... of 32 keys of the piece; the waves' states meet in LDS.
 // Per tile, on the 16x16x32 MFMA (bf16 or fp16, fp32 sums):
 //   S^T [32 keys, 16 rows] = K Q^T: the key rows as A fragments from LDS, the rows' queries held as B fragments;
@@ -38,9 +38,9 @@ struct Few {
 // after that are read one tile ahead, lane l for key l % 32, and handed to the loading lanes by ds_bpermute. Keys that no
 // row sees (past the piece, in a missing page) read a row of zeros. A value that some rows must not see could still be an
 // infinity or NaN (0 * inf): the waves look for it in the tiles that can hold one (row_by_keys).
-template <class T, int QF, int NW, int NKQ, int NT, bool PAGED>
+template <class T, int NW, int NKQ, int NT, bool PAGED>
 __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
-  using P = Few<QF, NW, NKQ, NT>;
+  using P = Few<NW, NKQ, NT>;
   constexpr int BR = P::BR;
   extern __shared__ __align__(16) char s_few[];
   const int tid = threadIdx.x, lane = lane_id();
@@ -126,32 +126,25 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   const int vfr = 4 * lq + lr / 4;
   const int vplace = vfr * P::VC * 16 + v_chunk_at<P::VC>(vfr, (lr % 4) / 2) * 16 + (lr & 1) * 8;
 
-  uint4 qf[QF][NKQ];
-  int lim[QF];  // keys that this lane's row sees
-#pragma unroll
-  for (int f = 0; f < QF; ++f) {
-    const int r = r0 + min(16 * f + lr, rows - 1), i = static_cast<int>(div_by(r, a.group));
-    const uint16_t* qrow = a.q.at(w.s.first + i, kvh * G + (r - i * G));
-    lim[f] = w.s.kv - w.s.n + i + 1;
+  uint4 qf[NKQ];
+  const int my_row = r0 + min(lr, rows - 1), my_i = static_cast<int>(div_by(my_row, a.group));
+  const int lim = w.s.kv - w.s.n + my_i + 1;  // keys that this lane's row sees
+  {
+    const uint16_t* qrow = a.q.at(w.s.first + my_i, kvh * G + (my_row - my_i * G));
+    const uint32_t sign = a.negative ? 0x80008000u : 0u;
 #pragma unroll
     for (int kk = 0; kk < NKQ; ++kk) {
       const int d = 32 * kk + 8 * lq;
       const bool ok = d < a.dqk;
-      uint4 x = and_mask16(ld16(qrow + (ok ? d : 0)), ok);
-      const uint32_t sign = a.negative ? 0x80008000u : 0u;
-      qf[f][kk] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+      const uint4 x = and_mask16(ld16(qrow + (ok ? d : 0)), ok);
+      qf[kk] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
     }
   }
   const int lim_all = w.s.kv - w.s.n + static_cast<int>(div_by(r0, a.group)) + 1;  // keys that every row sees
-  floatx4 o[QF][NT];
-  float m[QF], l[QF];
+  floatx4 o[NT];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int f = 0; f < QF; ++f) {
-    m[f] = -INFINITY;
-    l[f] = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) o[f][nt] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int nt = 0; nt < NT; ++nt) o[nt] = floatx4{0.f, 0.f, 0.f, 0.f};
   const float sc = a.scale * 1.4426950408889634f;  // scores in units of log2: exp2 gives the weights
   uint32_t seen = 0;  // exponents of values that some row must not meet
   if (wave < tiles) {
@@ -180,48 +173,40 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
         if constexpr (PAGED) next = page_id(a, w.b, key_of(it + 2 * NW));
         load_k();
       }
-      floatx4 s[QF][2];
-#pragma unroll
-      for (int f = 0; f < QF; ++f) s[f][0] = s[f][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+      floatx4 s[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int kk = 0; kk < NKQ; ++kk)
 #pragma unroll
-        for (int f = 0; f < QF; ++f)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) s[f][u] = Mfma<T>::m16(kx[u][kk], qf[f][kk], s[f][u]);
+        for (int u = 0; u < 2; ++u) s[u] = Mfma<T>::m16(kx[u][kk], qf[kk], s[u]);
       const bool mixed = j0 + kKeys > lim_all;  // some row does not see some key: its value must be finite, or 0 * inf reaches the row
-      uint4 pf[QF];
+      const int n = lim - j0;
+      const uint32_t sees = n >= kKeys ? mine : n <= 0 ? 0u : mine & ((1u << n) - 1u);
+      const uint32_t lo4 = sees >> (4 * lq), hi4 = sees >> (16 + 4 * lq);
+      float sv[8];
+      float tmax = -INFINITY;
 #pragma unroll
-      for (int f = 0; f < QF; ++f) {
-        const int n = lim[f] - j0;
-        const uint32_t sees = n >= kKeys ? mine : n <= 0 ? 0u : mine & ((1u << n) - 1u);
-        const uint32_t lo4 = sees >> (4 * lq), hi4 = sees >> (16 + 4 * lq);
-        float sv[8];
-        float tmax = -INFINITY;
+      for (int e = 0; e < 8; ++e) {  // slot e < 4 is key 4 lq + e of the tile, slot e >= 4 key 16 + 4 lq + e - 4
+        const bool see = e < 4 ? (lo4 >> e) & 1u : (hi4 >> (e - 4)) & 1u;
+        sv[e] = see ? (e < 4 ? s[0][e] : s[1][e - 4]) * sc : -INFINITY;
+        tmax = larger(tmax, sv[e]);
+      }
+      const float mn = fmaxf(m, quarter_max(tmax));
+      const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
+      const float alpha = exp2_fast(m - mu);
+      m = mn;
+      float ps = 0.f;
+      uint32_t pw[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {  // slot e < 4 is key 4 lq + e of the tile, slot e >= 4 key 16 + 4 lq + e - 4
-          const bool see = e < 4 ? (lo4 >> e) & 1u : (hi4 >> (e - 4)) & 1u;
-          sv[e] = see ? (e < 4 ? s[f][0][e] : s[f][1][e - 4]) * sc : -INFINITY;
-          tmax = larger(tmax, sv[e]);
-        }
-        const float mn = fmaxf(m[f], quarter_max(tmax));
-        const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
-        const float alpha = exp2_fast(m[f] - mu);
-        m[f] = mn;
-        float ps = 0.f;
-        uint32_t pw[4];
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = exp2_fast(sv[2 * e] - mu), p1 = exp2_fast(sv[2 * e + 1] - mu);
+        ps += p0 + p1;
+        pw[e] = pack2<T>(p0, p1);
+      }
+      l = fmaf(l, alpha, ps);
+      const uint4 pf = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+      if (__any(alpha != 1.f)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = exp2_fast(sv[2 * e] - mu), p1 = exp2_fast(sv[2 * e + 1] - mu);
-          ps += p0 + p1;
-          pw[e] = pack2<T>(p0, p1);
-        }
-        l[f] = fmaf(l[f], alpha, ps);
-        pf[f] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
-        if (__any(alpha != 1.f)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) o[f][nt] *= alpha;
-        }
+        for (int nt = 0; nt < NT; ++nt) o[nt] *= alpha;
       }
       if (more) wait_vmcnt<P::KI>();  // the tile's values (the next tile's keys still in flight)
       else wait_vmcnt<0>();
@@ -238,8 +223,7 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
           const uint4 vf = make_uint4(static_cast<uint32_t>(lo[b]), static_cast<uint32_t>(lo[b] >> 32),
                                       static_cast<uint32_t>(hi[b]), static_cast<uint32_t>(hi[b] >> 32));
           if (mixed) seen = add_exponents<T>(seen, vf);
-#pragma unroll
-          for (int f = 0; f < QF; ++f) o[f][n0 + b] = Mfma<T>::m16(vf, pf[f], o[f][n0 + b]);
+          o[n0 + b] = Mfma<T>::m16(vf, pf, o[n0 + b]);
         }
       }
       wait_lgkm0();  // read before the next tile overwrites them
@@ -249,17 +233,13 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   // the wave's state into its own LDS region, then the merge
   float* so = reinterpret_cast<float*>(s_few + wave * P::WAVE_BYTES);
   wave_lds_fence();
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
 #pragma unroll
-  for (int f = 0; f < QF; ++f) {
-    l[f] += __shfl_xor(l[f], 16, kWave);
-    l[f] += __shfl_xor(l[f], 32, kWave);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      *reinterpret_cast<floatx4*>(so + (16 * f + lr) * P::OROW + 16 * nt + 4 * lq) = o[f][nt];
-    if (lq == 0) {
-      so[P::ML + 16 * f + lr] = m[f];
-      so[P::ML + BR + 16 * f + lr] = l[f];
-    }
+  for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<floatx4*>(so + lr * P::OROW + 16 * nt + 4 * lq) = o[nt];
+  if (lq == 0) {
+    so[P::ML + lr] = m;
+    so[P::ML + BR + lr] = l;
   }
   const bool mine_met = __any((seen & kNotFinite) != 0);
   if (lane == 0) so[P::MET] = mine_met ? 1.f : 0.f;
@@ -434,8 +414,8 @@ int launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char
 
 template <class T, int NW, int NKQ, int NT, bool PAGED>
 int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
-  using P = Few<1, NW, NKQ, NT>;
-  auto kern = few_kernel<T, 1, NW, NKQ, NT, PAGED>;
+  using P = Few<NW, NKQ, NT>;
+  auto kern = few_kernel<T, NW, NKQ, NT, PAGED>;
   int rc = mm::allow_lds(kern, P::LDS, what);
   if (rc) return rc;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)), dim3(NW * kWave), P::LDS, st, a);
@@ -481,7 +461,8 @@ int64_t state_bytes(int64_t target, int nkv, int br, int dv) { return 2 * target
 // 16 streams behind 4000 to 40000 positions: 397 us uncut, 239 at 1 piece a CU, 217 at 2, 206 at 4, 202 at 8). Many rows over
 // a cache: 2 pieces a CU of at least 4 granules (pieces of 100 to 500 tokens behind 611 to 5000 positions: 149 us uncut, 98
 // at 1, 91 at 2, 101 at 3, 103 at 4; 512 tokens behind 30000: 798 uncut, 414, 316, 386 at 2.5). Prompts, whose keys are
-// their own tokens, only where their row blocks leave half of the CUs idle (12 ragged Talker prompts: 42 us uncut, 47 cut).
+// their own tokens, only where their row blocks leave half of the CUs idle and can be long (2 heads of 64, 2000 tokens: 24.8
+// us uncut, 15.6 cut; 12 ragged Talker prompts: 42 and 47; 300 tokens of 32/8 heads of 128: 14.0 and 16.5).
 // Two groups of waves to a block where a prompt's blocks are fewer than 4 a CU: they halve the time of the last block (12
 // ragged Talker prompts 42.8 -> 38.5 us, 2000 Talker tokens 37.4 -> 29.6, 4000 72 -> 59), but in a long run two workgroups
 // of one group mix matrix and vector work better (8192 tokens of 32/8 heads of 128: 590 | 643), and over a cache the cut
@@ -492,7 +473,7 @@ AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, i
   p.many = rows > 16 * seqs && reads_of_few(rows, seqs, max_keys, nkv, dqk, dv) > kFewReads;
   p.blocks = most_blocks(rows, seqs, p.many ? 128 : 16);
   if (p.many) {
-    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus) p.target = many_target(nkv);
+    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus && max_keys > 1024) p.target = many_target(nkv);
     p.groups = !paged && p.target == 0 && p.blocks * nkv < 4 * cus && dqk <= 192 && dv <= 128 ? 2 : 1;
     p.workspace = state_bytes(p.target, nkv, 128, dv);
   } else {

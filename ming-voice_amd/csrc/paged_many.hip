@@ -1,5 +1,5 @@
-// Attention of many rows (prompts and their pieces): 128 rows to a workgroup of four waves that share every key and value
-// tile in LDS.
+// Attention of many rows (prompts and their pieces): 128 rows to a workgroup whose waves share every key and value tile in
+// LDS.
 #include "paged_common.h"
 
 namespace mmp {
@@ -44,8 +44,33 @@ __device__ __forceinline__ float half_max(float v) {
   return larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Where a tile's rows come from, chosen on the host (rows_of_kind).
+// Where a tile's rows come from, chosen on the host (launch_type).
 enum Source { kPacked, kPaged, kAnywhere };
+
+// Softmax attention of 128 rows over a piece of their keys (all of them, where the batch is not cut), one pass with a
+// running maximum and sum. Grid (work x key / value heads) x NG groups of 4 waves; a wave holds 32 rows, a group goes
+// through 64 keys at a time, which its waves share in LDS, and two groups take every other tile and join their states in LDS
+// at the end. Per tile and wave, on the 32x32x16 MFMA (bf16 or fp16, fp32 sums):
+//   S^T [64 keys, 32 rows] = K Q^T: key rows as A fragments from LDS, the queries held as B fragments;
+//   a lane of S^T holds 32 keys of row lane % 32, so that maximum, exponentials and sum need one exchange, with lane ^ 32;
+//   O^T [dv, 32 rows] += V^T P^T: P^T straight from the S^T registers (slot j of step st is the key of S^T register 8 (st % 2)
+//     + j, whichever that is, for both operands alike), the weights rounded to the cache's type, the matrix units' operand
+//     (half a step, 2^-9 of a weight in bf16); V^T by transposing LDS reads.
+// The running maximum follows a tile's only when it rises by more than 2^8 in weight: the sums of a row then stay below 2^8
+// times their final size, far inside fp32 and inside fp16's and bf16's weights, and O is seldom rescaled.
+// A tile comes by loads straight into LDS while the tile before is computed: one barrier a tile, after which the wave
+// requests its part of the next one (8 rows by 128 bytes an instruction). Swizzles keep every LDS read free of bank
+// conflicts (SQ_LDS_BANK_CONFLICT 0). All key fragments are read before the first product and all value fragments before
+// the softmax, so that neither waits for LDS.
+// Bound by how far matrix and vector work of the two workgroups of a CU overlap: at 8192 tokens of 32/8 heads of 128 (550
+// GFLOP of pairs that count) 549 us, 1.0 PFLOP/s, where the 8192^3 product runs at 1.15; the matrix units are busy 55 % of
+// the cycles, the vector units 50 %. At 64 dims the exponentials (a quarter of the vector rate) and 4 more vector
+// instructions a score weigh as much as the products twice: 12 Talker prompts of 5 to 2000 tokens 31.7 us (357 TFLOP/s),
+// 4000 tokens 52 us. On the way there (8192 tokens): 932 us with rows brought by ds_bpermute and fragments read one by one;
+// 673 with 64-dim pieces, one page to a load and the not-finite code out of the loop; 616 with the key fragments ahead, 588
+// with the value fragments too; 560 with one instruction to a pair of weights and to two of a maximum. Not kept: s_setprio
+// around the products (588 -> 600), exponentials dealt out between the products (627), for 256 dims the value fragments
+// ahead (spills).
 
 template <class T, int KS, int VS, int NG, int SRC>
 __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(AttnArgs a) {
