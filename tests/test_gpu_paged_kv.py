@@ -59,6 +59,26 @@ class Streams:
         return O.paged_attn(self.q[:self.N], self.kp, self.vp, self.table, self.cu, self.lens, scale or self.dqk ** -0.5)
 
 
+# The host chooses the kernel by the sizes alone: blocks of 16 rows where these would read few keys, of 128 rows (in one or
+# two groups of waves) where many. The same small batch goes through each of them by a table that allows long contexts, and
+# by rows behind the last prompt.
+WIDE_TABLE = 400000  # positions
+
+
+def many_pages(kind, page):
+    return 2 if kind == "few" else WIDE_TABLE // page
+
+
+def spare_rows(kind, nh, dqk, dv):
+    if kind == "few":
+        return 3
+    return 300 + (131072 // nh if kind == "one group" else int(((64 << 20) * 16 / (nh * (dqk + dv) * 2)) ** 0.5))
+
+
+BOTH = pytest.mark.parametrize("kind", ["few", "many"])
+ALL = pytest.mark.parametrize("kind", ["few", "one group", "two groups"])
+
+
 def check(got, want, keys, dqk, dtype):
     out, wv, mag = want
     tol = O.attn_tolerance(out, wv, mag, keys, dqk, dtype)
@@ -156,9 +176,11 @@ def test_append_stores_nothing_where_nothing_exists():
                                                    (BF, torch.int32, 1000, "hnd")])
 @pytest.mark.parametrize("new,ctx", [([1, 1, 1, 1, 1], [0, 1, 63, 64, 300]), ([5, 1, 0, 37, 2], [0, 700, 9, 130, 31]),
                                      ([150], [45]), ([1], [0])])
-def test_paged_attn(nh, nkv, dqk, dv, dtype, idx, page, layout, new, ctx):
-    print(f"heads {nh}/{nkv} {dqk}/{dv} {dtype} {idx} page {page} {layout} {new} behind {ctx}", flush=True)
-    s = Streams(new, ctx, nh, nkv, dqk, dv, page, dtype, idx, seed=len(new), layout=layout)
+@BOTH
+def test_paged_attn(nh, nkv, dqk, dv, dtype, idx, page, layout, new, ctx, kind):
+    print(f"heads {nh}/{nkv} {dqk}/{dv} {dtype} {idx} page {page} {layout} {new} behind {ctx} {kind}", flush=True)
+    s = Streams(new, ctx, nh, nkv, dqk, dv, page, dtype, idx, seed=len(new), layout=layout,
+                more_pages=many_pages(kind, page))
     got = s.attn()
     check(got, s.oracle(), max(s.kv), dqk, dtype)
 
@@ -175,10 +197,12 @@ def test_long_contexts(nh, nkv, dqk, dv, new, ctx):
 
 
 @pytest.mark.parametrize("count", [63, 64, 65, 130, 700])
-def test_many_streams(count):
-    new = [i % 3 for i in range(count)]
-    s = Streams(new, [(i * 37) % 90 for i in range(count)], 4, 2, 64, 64, page=8, seed=count)
-    check(s.attn(), s.oracle(), 100, 64, BF)
+@BOTH
+def test_many_streams(count, kind):
+    new = [(0, 1, 30)[i % 3] if kind == "many" else i % 3 for i in range(count)]
+    s = Streams(new, [(i * 37) % 90 + 700 * (i == 5) for i in range(count)], 4, 2, 64, 64, page=8, seed=count,
+                more_pages=many_pages(kind, 8))
+    check(s.attn(), s.oracle(), 900, 64, BF)
 
 
 def test_every_token_a_stream_of_its_own_or_none():
@@ -190,8 +214,9 @@ def test_every_token_a_stream_of_its_own_or_none():
     assert (out == 5.0).all()
 
 
-def test_rows_that_see_nothing_are_zero_and_bad_lengths_nan():
-    s = Streams([4, 3, 2, 5, 1, 2], [30, 6, 20, 1, 10, 0], seed=11, spare=4)
+@BOTH
+def test_rows_that_see_nothing_are_zero_and_bad_lengths_nan(kind):
+    s = Streams([4, 3, 2, 5, 1, 2], [30, 6, 20, 1, 10, 0], seed=11, spare=4, more_pages=many_pages(kind, 16))
     s.lens[0] = 2                                          # tokens 0, 1 stand before position 0
     s.lens[1] = s.table.shape[1] * s.page + 1
     s.lens[2] = -1
@@ -209,19 +234,21 @@ def test_rows_that_see_nothing_are_zero_and_bad_lengths_nan():
 
 @pytest.mark.parametrize("page", [4, 32, 100])
 @pytest.mark.parametrize("new", [[1, 1], [40, 3], [200, 1]])
-def test_missing_pages_are_left_out(page, new):
-    s = Streams(new, [400, 77], page=page, seed=13)
-    for at in range(0, s.table.shape[1], 3):
+@BOTH
+def test_missing_pages_are_left_out(page, new, kind):
+    s = Streams(new, [400, 77], page=page, seed=13, more_pages=many_pages(kind, page))
+    for at in range(0, -(-s.kv[0] // page), 3):
         s.table[0, at] = -1 if at % 2 else 1 << 30
     check(s.attn(), s.oracle(), 700, 64, BF)
 
 
 @pytest.mark.parametrize("nh,nkv,dqk,dv", [(14, 2, 64, 64), (4, 2, 128, 128), (2, 2, 192, 128), (4, 2, 256, 256), (6, 2, 80, 80)])
-@pytest.mark.parametrize("new,ctx", [([7], [0]), ([90, 1], [3, 40]), ([300], [100])])
+@pytest.mark.parametrize("new,ctx", [([7], [0]), ([90, 1], [3, 40]), ([300], [1000])])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_later_rows_never_reach_a_token(nh, nkv, dqk, dv, new, ctx, bad):
+@BOTH
+def test_later_rows_never_reach_a_token(nh, nkv, dqk, dv, new, ctx, bad, kind):
     """What the last two positions of a stream hold is seen by its last two tokens alone."""
-    s = Streams(new, ctx, nh, nkv, dqk, dv, seed=17)
+    s = Streams(new, ctx, nh, nkv, dqk, dv, seed=17, more_pages=many_pages(kind, 16))
     want = s.oracle()
     for b, kv in enumerate(s.kv):
         for p in (kv - 2, kv - 1):
@@ -239,17 +266,19 @@ def test_later_rows_never_reach_a_token(nh, nkv, dqk, dv, new, ctx, bad):
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0, 1e-6])
 @pytest.mark.parametrize("dtype", [BF, FP])
-def test_scales(scale, dtype):
-    s = Streams([1, 40, 200], [90, 17, 0], dtype=dtype, seed=19)
+@BOTH
+def test_scales(scale, dtype, kind):
+    s = Streams([1, 40, 200], [90, 17, 0], dtype=dtype, seed=19, more_pages=many_pages(kind, 16))
     got = s.attn(scale=scale)
     want = O.paged_attn(s.q, s.kp, s.vp, s.table, s.cu, s.lens, scale)
     check(got, want, 300, 64, dtype)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
-def test_weights_far_apart(dtype):
+@BOTH
+def test_weights_far_apart(dtype, kind):
     """Scores that rise and fall by hundreds along the keys: the running maximum moves often."""
-    s = Streams([1, 64, 130], [1500, 700, 20], dtype=dtype, seed=23, std=4.0)
+    s = Streams([1, 64, 130], [1500, 700, 20], dtype=dtype, seed=23, std=4.0, more_pages=many_pages(kind, 16))
     check(s.attn(scale=1.0), s.oracle(1.0), 1600, 64, dtype)
 
 
@@ -281,22 +310,37 @@ def test_offsets_past_32_bits():
     assert torch.equal(far_v.nan_to_num(7.0), s.vp.nan_to_num(7.0))
 
 
+def test_rows_far_apart_in_a_block_of_many_rows():
+    """Keys and values 128 MiB apart, past what one buffer resource spans, at 512 query heads on one."""
+    s = Streams([70, 30], [0, 0], nh=512, nkv=1, seed=30)
+    gap = 1 << 26
+    raw = torch.empty(s.N * gap, device=DEV, dtype=BF)
+    k, v = (raw.as_strided((s.N, 1, 64), (gap, 64, 1), 64 * i) for i in range(2))
+    k.copy_(s.k)
+    v.copy_(s.v)
+    got = PK.prompt_attn(s.q, k, v, s.cu)
+    assert torch.equal(got, PK.prompt_attn(s.q, s.k, s.v, s.cu))
+    check(got, O.prompt_attn(s.q, s.k, s.v, s.cu, 0.125), 70, 64, BF)
+
+
 # ------------------------------------------------------------------------------------------------ packed prompts
 
 @pytest.mark.parametrize("nh,nkv,dqk,dv", HEADS)
 @pytest.mark.parametrize("dtype,idx", [(BF, torch.int32), (FP, torch.int64)])
 @pytest.mark.parametrize("new", [[1], [2, 0, 31, 1], [64, 65, 3], [300], [17] * 9])
-def test_prompt_attn(nh, nkv, dqk, dv, dtype, idx, new):
-    print(f"heads {nh}/{nkv} {dqk}/{dv} {dtype} {new}", flush=True)
-    s = Streams(new, [0] * len(new), nh, nkv, dqk, dv, dtype=dtype, idx=idx, seed=31, spare=3)
-    out = torch.full((s.N + 3, nh, dv), 9.0, device=DEV, dtype=dtype)
+@ALL
+def test_prompt_attn(nh, nkv, dqk, dv, dtype, idx, new, kind):
+    print(f"heads {nh}/{nkv} {dqk}/{dv} {dtype} {new} {kind}", flush=True)
+    s = Streams(new, [0] * len(new), nh, nkv, dqk, dv, dtype=dtype, idx=idx, seed=31, spare=spare_rows(kind, nh, dqk, dv))
+    out = torch.full((len(s.q), nh, dv), 9.0, device=DEV, dtype=dtype)
     assert PK.prompt_attn(s.q, s.k, s.v, s.cu, out=out) is out
     check(out[:s.N], O.prompt_attn(s.q[:s.N], s.k[:s.N], s.v[:s.N], s.cu, dqk ** -0.5), max(new), dqk, dtype)
     assert (out[s.N:] == 9.0).all()
 
 
 @pytest.mark.parametrize("nh,nkv,dqk,dv,new", [(14, 2, 64, 64, [1500, 3, 700]), (4, 1, 128, 128, [2100]),
-                                               (2, 2, 192, 128, [900, 901]), (2, 1, 256, 256, [1030])])
+                                               (2, 2, 192, 128, [900, 901]), (2, 1, 256, 256, [1030]),
+                                               (2, 2, 64, 64, [2300]), (32, 8, 128, 128, [1500, 2600])])
 def test_long_prompts(nh, nkv, dqk, dv, new):
     s = Streams(new, [0] * len(new), nh, nkv, dqk, dv, seed=37)
     got = PK.prompt_attn(s.q, s.k, s.v, s.cu)
@@ -306,13 +350,20 @@ def test_long_prompts(nh, nkv, dqk, dv, new):
 
 @pytest.mark.parametrize("new", [[9, 40], [300, 77]])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_other_prompts_never_reach_a_token(new, bad):
-    s = Streams(new, [0, 0], seed=41)
+@ALL
+def test_other_prompts_and_later_tokens_never_reach_a_token(new, bad, kind):
+    s = Streams(new, [0, 0], seed=41, spare=spare_rows(kind, 14, 64, 64))
     want = PK.prompt_attn(s.q, s.k, s.v, s.cu)
+    v = s.v.clone()
+    v[new[0] - 3:new[0]] = bad  # the first prompt's last three: seen by those tokens alone
+    got = PK.prompt_attn(s.q, s.k, v, s.cu)
+    check(got[:new[0] - 3], tuple(o[:new[0] - 3] for o in O.prompt_attn(s.q[:s.N], s.k[:s.N], s.v[:s.N], s.cu, 0.125)),
+          max(new), 64, BF)
+    assert torch.equal(got[new[0]:s.N], want[new[0]:s.N]) and not got[new[0] - 1].isfinite().any()
     for first, count, keep in ((0, new[0], slice(new[0], None)), (new[0], new[1], slice(0, new[0]))):
         k, v = s.k.clone(), s.v.clone()
         k[first:first + count], v[first:first + count] = bad, bad
-        assert torch.equal(PK.prompt_attn(s.q, k, v, s.cu)[keep], want[keep])
+        assert torch.equal(PK.prompt_attn(s.q, k, v, s.cu)[:s.N][keep], want[:s.N][keep])
 
 
 def test_broadcast_and_strided_inputs():
@@ -471,10 +522,11 @@ def test_no_streams_no_tokens_no_pages():
     assert none.shape == (0, 4, 64)
 
 
-def test_indices_that_make_no_sense_stay_in_bounds():
+@BOTH
+def test_indices_that_make_no_sense_stay_in_bounds(kind):
     """cu_seqlens that falls, starts behind 0 or ends behind the tokens: which rows are computed is open, but every access
     stays inside the tensors (the host-side twin of the work's division: tests/test_paged_kv.py)."""
-    s = Streams([5, 60, 3], [100, 900, 0], seed=83)
+    s = Streams([5, 60, 3], [100, 900, 0], seed=83, more_pages=many_pages(kind, 16))
     for cu in ([0, 65, 5, 68], [3, 5, 65, 68], [0, 5, 65, 9999], [-7, 5, 65, 68], [68, 0, 68, 0], [0, 68, 0, 68]):
         s.cu = torch.tensor(cu, device=DEV, dtype=torch.int32)
         s.attn()
