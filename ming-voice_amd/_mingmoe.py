@@ -6,6 +6,7 @@ shared). There is no fallback: if the library is missing or a call fails, a Runt
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -50,14 +51,48 @@ class Pages(ctypes.Structure):
                 ("dv", ctypes.c_int32), ("n_pages", _I64), ("page", _I64), ("k_page_stride", _I64),
                 ("k_head_stride", _I64), ("k_row_stride", _I64), ("v_page_stride", _I64), ("v_head_stride", _I64),
                 ("v_row_stride", _I64)]
-    _as_parameter_ = property(ctypes.byref)
 
 
 class Batch(ctypes.Structure):
     """mm_batch: packed tokens of several streams (cu, kv_lens and the page table, device arrays of one dtype)."""
     _fields_ = [("cu", _P), ("kv_lens", _P), ("table", _P), ("table_stride", _I64), ("max_pages", _I64),
                 ("seqs", _I64), ("tokens", _I64), ("idx_dtype", ctypes.c_int32)]
-    _as_parameter_ = property(ctypes.byref)
+
+
+class Rows(ctypes.Structure):
+    """mm_rows: rows [tokens, heads, d] of a packed tensor."""
+    _fields_ = [("p", _P), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """mm_paged_append_args."""
+    _fields_ = [("pages", Pages), ("batch", Batch), ("q", Rows), ("k", Rows), ("v", Rows), ("q_out", Rows),
+                ("k_out", Rows), ("inv_freq", _P), ("pairs", _I64), ("nh", ctypes.c_int32),
+                ("rot_offset", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """mm_paged_attn_args."""
+    _fields_ = [("pages", Pages), ("batch", Batch), ("q", Rows), ("out", Rows), ("workspace", _P),
+                ("workspace_bytes", _I64), ("nh", ctypes.c_int32), ("scale", _F32)]
+
+
+class PromptAttnArgs(ctypes.Structure):
+    """mm_prompt_attn_args."""
+    _fields_ = [("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("cu", _P), ("seqs", _I64), ("tokens", _I64),
+                ("workspace", _P), ("workspace_bytes", _I64), ("idx_dtype", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("nh", ctypes.c_int32), ("nkv", ctypes.c_int32), ("dqk", ctypes.c_int32), ("dv", ctypes.c_int32),
+                ("scale", _F32)]
+
+
+def packer(structure):
+    """A struct.Struct that packs the fields of a ctypes structure, nested ones in line, as C lays them out (no pointer is
+    None): an argument block in one call, where filling the structure takes one a field."""
+    codes = {_P: "P", _I64: "q", ctypes.c_int32: "i", _F32: "f"}
+
+    def fields(s):
+        return "".join(fields(f) + "0q" if issubclass(f, ctypes.Structure) else codes[f] for _, f in s._fields_)
+    return struct.Struct("@" + fields(structure) + "0q")
 
 
 SIGNATURES = {
@@ -119,16 +154,14 @@ SIGNATURES = {
 }
 
 # the entry points of include/mingpaged.h
-PAGED_VERSION = 1
+PAGED_VERSION = 2
 PAGED_SIGNATURES = {
     "mm_paged_version": ([], ctypes.c_int),
-    "mm_paged_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P], ctypes.c_int),
+    "mm_paged_append": ([_P, _P], ctypes.c_int),
     "mm_paged_attn_workspace": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32], _I64),
-    "mm_paged_attn": ([_P, _I64, _I64, _I32, _P, _P, _F32, _P, _I64, _I64, _P,
-                       _I64, _P], ctypes.c_int),
+    "mm_paged_attn": ([_P, _P], ctypes.c_int),
     "mm_prompt_attn_workspace": ([_I64, _I64, _I32, _I32, _I32, _I32, _I32], _I64),
-    "mm_prompt_attn": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64,
-                        _I64, _F32, _P, _I64, _I64, _P, _I64, _P], ctypes.c_int),
+    "mm_prompt_attn": ([_P, _P], ctypes.c_int),
 }
 
 _lib = None

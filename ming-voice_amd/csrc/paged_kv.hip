@@ -174,10 +174,10 @@ constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxPages = (1LL << 
 // positions of a stream, and rows (tokens times heads): 32-bit numbers of them stay positive with a tile or a piece added
 constexpr int64_t kMaxKeys = 1LL << 30, kMaxRows = 1LL << 30;
 
-// A row of strides; those of a dim of one are not used and may be anything.
-int check_rows(const char* what, const char* name, const void* p, int64_t tokens, int64_t ts, int heads, int64_t hs, int align) {
-  MM_REQUIRE(p, "%s: null %s", what, name);
-  MM_REQUIRE((reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(align - 1)) == 0, "%s: %s must be %d-byte aligned",
+int check_rows(const char* what, const char* name, const mm_rows& r, int64_t tokens, int heads, int align) {
+  const int64_t ts = r.token_stride, hs = r.head_stride;
+  MM_REQUIRE(r.p, "%s: null %s", what, name);
+  MM_REQUIRE((reinterpret_cast<uintptr_t>(r.p) & static_cast<uintptr_t>(align - 1)) == 0, "%s: %s must be %d-byte aligned",
              what, name, align);
   MM_REQUIRE((tokens == 1 || (ts >= 0 && ts % (align / 2) == 0)) && (heads == 1 || (hs >= 0 && hs % (align / 2) == 0)),
              "%s: strides of %s must keep rows %d-byte aligned", what, name, align);
@@ -200,7 +200,6 @@ int check_tokens(const char* what, int64_t tokens, int64_t seqs) {
 }
 
 int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) {
-  MM_REQUIRE(g && b, "%s: null descriptor", what);
   int rc = check_shape(what, g->dtype, nh, g->nkv, g->dqk, g->dv);
   if (rc) return rc;
   if ((rc = check_tokens(what, b->tokens, b->seqs))) return rc;
@@ -218,16 +217,20 @@ int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) 
   return MM_OK;
 }
 
-Batch batch_of(const mm_pages* g, const mm_batch* b) {
-  return Batch{b->cu, b->kv_lens, b->table, b->table_stride, b->idx_dtype == MM_INT64, static_cast<int>(b->seqs),
-               static_cast<int>(b->tokens), static_cast<int>(b->max_pages * g->page)};
+Batch batch_of(const mm_pages& g, const mm_batch& b) {
+  return Batch{b.cu, b.kv_lens, b.table, b.table_stride, b.idx_dtype == MM_INT64, static_cast<int>(b.seqs),
+               static_cast<int>(b.tokens), static_cast<int>(b.max_pages * g.page)};
 }
 
-Rows rows_of(const void* p, int64_t ts, int64_t hs) { return Rows{static_cast<uint16_t*>(const_cast<void*>(p)), ts, hs}; }
+Rows rows_of(const mm_rows& r) { return Rows{static_cast<uint16_t*>(r.p), r.token_stride, r.head_stride}; }
 
-void set_pool(const mm_pages* g, Pool& k, Pool& v) {
-  k = Pool{static_cast<uint16_t*>(g->k), g->k_page_stride, g->k_head_stride, g->k_row_stride};
-  v = Pool{static_cast<uint16_t*>(g->v), g->v_page_stride, g->v_head_stride, g->v_row_stride};
+bool same_rows(const mm_rows& a, const mm_rows& b) {
+  return a.p == b.p && a.token_stride == b.token_stride && a.head_stride == b.head_stride;
+}
+
+void set_pool(const mm_pages& g, Pool& k, Pool& v) {
+  k = Pool{static_cast<uint16_t*>(g.k), g.k_page_stride, g.k_head_stride, g.k_row_stride};
+  v = Pool{static_cast<uint16_t*>(g.v), g.v_page_stride, g.v_head_stride, g.v_row_stride};
 }
 
 int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int64_t workspace_bytes, hipStream_t st,
@@ -249,49 +252,45 @@ int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int
 
 extern "C" int mm_paged_version(void) { return MM_PAGED_VERSION; }
 
-extern "C" int mm_paged_append(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
-                               const void* v, int64_t v_ts, int64_t v_hs, int nh, const mm_pages* pages,
-                               const mm_batch* batch, const float* inv_freq, int64_t pairs, int rot_offset, int interleaved,
-                               void* q_out, int64_t qo_ts, int64_t qo_hs, void* k_out, int64_t ko_ts, int64_t ko_hs,
-                               void* stream) {
+extern "C" int mm_paged_append(const mm_paged_append_args* g, void* stream) {
   const char* what = "paged_append";
-  int rc = check_paged(what, nh, pages, batch);
+  MM_REQUIRE(g, "%s: null arguments", what);
+  int rc = check_paged(what, g->nh, &g->pages, &g->batch);
   if (rc) return rc;
-  if (!inv_freq) pairs = rot_offset = 0;
+  const int64_t pairs = g->inv_freq ? g->pairs : 0;
+  const int rot_offset = g->inv_freq ? g->rot_offset : 0, nkv = g->pages.nkv;
   MM_REQUIRE(pairs >= 0 && pairs % 8 == 0 && rot_offset >= 0 && rot_offset % 8 == 0 && pairs <= kMaxPairs &&
-                 rot_offset + 2 * pairs <= pages->dqk,
+                 rot_offset + 2 * pairs <= g->pages.dqk,
              "paged_append: %lld pairs from dim %d on do not fit a head of %d (multiples of 8)", (long long)pairs, rot_offset,
-             pages->dqk);
-  const int64_t N = batch->tokens;
-  const int nkv = pages->nkv;
-  if (N == 0 || batch->seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, N, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "k", k, N, k_ts, nkv, k_hs, 16)) ||
-      (rc = check_rows(what, "v", v, N, v_ts, nkv, v_hs, 16)) ||
-      (rc = check_rows(what, "q_out", q_out, N, qo_ts, nh, qo_hs, 16)))
+             g->pages.dqk);
+  const int64_t N = g->batch.tokens;
+  if (N == 0 || g->batch.seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "k", g->k, N, nkv, 16)) ||
+      (rc = check_rows(what, "v", g->v, N, nkv, 16)) || (rc = check_rows(what, "q_out", g->q_out, N, g->nh, 16)))
     return rc;
-  if (k_out && (rc = check_rows(what, "k_out", k_out, N, ko_ts, nkv, ko_hs, 16))) return rc;
+  if (g->k_out.p && (rc = check_rows(what, "k_out", g->k_out, N, nkv, 16))) return rc;
   AppendArgs a{};
-  a.q = rows_of(q, q_ts, q_hs);
-  a.k = rows_of(k, k_ts, k_hs);
-  a.v = rows_of(v, v_ts, v_hs);
-  a.q_out = rows_of(q_out, qo_ts, qo_hs);
-  a.k_out = rows_of(k_out, ko_ts, ko_hs);
-  set_pool(pages, a.kp, a.vp);
-  a.batch = batch_of(pages, batch);
-  a.page = fast_div(pages->page);
-  a.n_pages = pages->n_pages;
-  a.inv_freq = inv_freq;
-  a.nh = nh;
+  a.q = rows_of(g->q);
+  a.k = rows_of(g->k);
+  a.v = rows_of(g->v);
+  a.q_out = rows_of(g->q_out);
+  a.k_out = rows_of(g->k_out);
+  set_pool(g->pages, a.kp, a.vp);
+  a.batch = batch_of(g->pages, g->batch);
+  a.page = fast_div(g->pages.page);
+  a.n_pages = g->pages.n_pages;
+  a.inv_freq = g->inv_freq;
+  a.nh = g->nh;
   a.nkv = nkv;
-  a.dqk = pages->dqk;
-  a.dv = pages->dv;
+  a.dqk = g->pages.dqk;
+  a.dv = g->pages.dv;
   a.pairs = static_cast<int>(pairs);
   a.rot_offset = rot_offset;
-  a.interleaved = interleaved != 0;
+  a.interleaved = g->interleaved != 0;
   a.iph = fast_div(a.pairs / 8 + (a.dqk - 2 * a.pairs) / 8);
-  a.q_in_place = q_out == q && qo_ts == q_ts && qo_hs == q_hs;
-  a.k_in_place = k_out == nullptr || (k_out == k && ko_ts == k_ts && ko_hs == k_hs);
-  return pages->dtype == MM_BF16 ? launch_append<BF16>(a, MM_STREAM(stream)) : launch_append<FP16>(a, MM_STREAM(stream));
+  a.q_in_place = same_rows(g->q_out, g->q);
+  a.k_in_place = g->k_out.p == nullptr || same_rows(g->k_out, g->k);
+  return g->pages.dtype == MM_BF16 ? launch_append<BF16>(a, MM_STREAM(stream)) : launch_append<FP16>(a, MM_STREAM(stream));
 }
 
 extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, int nh, int nkv, int dqk, int dv,
@@ -304,28 +303,27 @@ extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t
   return workspace_of(true, tokens, seqs, max_keys, nh, nkv, dqk, dv, at_most != 0);
 }
 
-extern "C" int mm_paged_attn(const void* q, int64_t q_ts, int64_t q_hs, int nh, const mm_pages* pages, const mm_batch* batch,
-                             float scale, void* out, int64_t o_ts, int64_t o_hs, void* workspace, int64_t workspace_bytes,
-                             void* stream) {
+extern "C" int mm_paged_attn(const mm_paged_attn_args* g, void* stream) {
   const char* what = "paged_attn";
-  int rc = check_paged(what, nh, pages, batch);
+  MM_REQUIRE(g, "%s: null arguments", what);
+  int rc = check_paged(what, g->nh, &g->pages, &g->batch);
   if (rc) return rc;
-  const int64_t N = batch->tokens;
-  if (N == 0 || batch->seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, N, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "out", out, N, o_ts, nh, o_hs, 8))) return rc;
+  const int64_t N = g->batch.tokens;
+  if (N == 0 || g->batch.seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8))) return rc;
   AttnArgs a{};
-  a.q = rows_of(q, q_ts, q_hs);
-  a.out = rows_of(out, o_ts, o_hs);
-  set_pool(pages, a.kp, a.vp);
-  a.batch = batch_of(pages, batch);
-  a.page = fast_div(pages->page);
-  a.group = fast_div(nh / pages->nkv);
-  a.n_pages = static_cast<int>(pages->n_pages);
-  a.nh = nh;
-  a.nkv = pages->nkv;
-  a.dqk = pages->dqk;
-  a.dv = pages->dv;
-  return attend(a, pages->dtype, true, scale, workspace, workspace_bytes, MM_STREAM(stream), what);
+  a.q = rows_of(g->q);
+  a.out = rows_of(g->out);
+  set_pool(g->pages, a.kp, a.vp);
+  a.batch = batch_of(g->pages, g->batch);
+  a.page = fast_div(g->pages.page);
+  a.group = fast_div(g->nh / g->pages.nkv);
+  a.n_pages = static_cast<int>(g->pages.n_pages);
+  a.nh = g->nh;
+  a.nkv = g->pages.nkv;
+  a.dqk = g->pages.dqk;
+  a.dv = g->pages.dv;
+  return attend(a, g->pages.dtype, true, g->scale, g->workspace, g->workspace_bytes, MM_STREAM(stream), what);
 }
 
 extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int dqk, int dv, int at_most) {
@@ -333,32 +331,31 @@ extern "C" int64_t mm_prompt_attn_workspace(int64_t tokens, int64_t seqs, int nh
   return workspace_of(false, tokens, seqs, tokens, nh, nkv, dqk, dv, at_most != 0);
 }
 
-extern "C" int mm_prompt_attn(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
-                              const void* v, int64_t v_ts, int64_t v_hs, int dtype, int nh, int nkv, int dqk, int dv,
-                              const void* cu, int idx_dtype, int64_t seqs, int64_t tokens, float scale, void* out,
-                              int64_t o_ts, int64_t o_hs, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int mm_prompt_attn(const mm_prompt_attn_args* g, void* stream) {
   const char* what = "prompt_attn";
-  int rc = check_shape(what, dtype, nh, nkv, dqk, dv);
+  MM_REQUIRE(g, "%s: null arguments", what);
+  const int64_t N = g->tokens;
+  int rc = check_shape(what, g->dtype, g->nh, g->nkv, g->dqk, g->dv);
   if (rc) return rc;
-  if ((rc = check_tokens(what, tokens, seqs))) return rc;
-  MM_REQUIRE(idx_dtype == MM_INT32 || idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
-  MM_REQUIRE(cu || seqs == 0, "%s: null cu", what);
-  MM_REQUIRE(tokens * nh <= kMaxRows, "%s: tokens * nh must be at most 2^30", what);
-  if (tokens == 0 || seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", q, tokens, q_ts, nh, q_hs, 16)) || (rc = check_rows(what, "k", k, tokens, k_ts, nkv, k_hs, 16)) ||
-      (rc = check_rows(what, "v", v, tokens, v_ts, nkv, v_hs, 16)) || (rc = check_rows(what, "out", out, tokens, o_ts, nh, o_hs, 8)))
+  if ((rc = check_tokens(what, N, g->seqs))) return rc;
+  MM_REQUIRE(g->idx_dtype == MM_INT32 || g->idx_dtype == MM_INT64, "%s: indices must be int32 or int64", what);
+  MM_REQUIRE(g->cu || g->seqs == 0, "%s: null cu", what);
+  MM_REQUIRE(N * g->nh <= kMaxRows, "%s: tokens * nh must be at most 2^30", what);
+  if (N == 0 || g->seqs == 0) return MM_OK;
+  if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "k", g->k, N, g->nkv, 16)) ||
+      (rc = check_rows(what, "v", g->v, N, g->nkv, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8)))
     return rc;
   AttnArgs a{};
-  a.q = rows_of(q, q_ts, q_hs);
-  a.k = rows_of(k, k_ts, k_hs);
-  a.v = rows_of(v, v_ts, v_hs);
-  a.out = rows_of(out, o_ts, o_hs);
-  a.batch = Batch{cu, nullptr, nullptr, 0, idx_dtype == MM_INT64, static_cast<int>(seqs), static_cast<int>(tokens), 0};
+  a.q = rows_of(g->q);
+  a.k = rows_of(g->k);
+  a.v = rows_of(g->v);
+  a.out = rows_of(g->out);
+  a.batch = Batch{g->cu, nullptr, nullptr, 0, g->idx_dtype == MM_INT64, static_cast<int>(g->seqs), static_cast<int>(N), 0};
   a.page = fast_div(1);
-  a.group = fast_div(nh / nkv);
-  a.nh = nh;
-  a.nkv = nkv;
-  a.dqk = dqk;
-  a.dv = dv;
-  return attend(a, dtype, false, scale, workspace, workspace_bytes, MM_STREAM(stream), what);
+  a.group = fast_div(g->nh / g->nkv);
+  a.nh = g->nh;
+  a.nkv = g->nkv;
+  a.dqk = g->dqk;
+  a.dv = g->dv;
+  return attend(a, g->dtype, false, g->scale, g->workspace, g->workspace_bytes, MM_STREAM(stream), what);
 }

@@ -21,19 +21,16 @@ and for prompts that start from nothing prompt_attn(q, k, v, cu_seqlens) with th
 call's place. Every call enqueues on torch's current stream of its tensors' device and can be captured in a hipGraph;
 there is no CPU path.
 """
-import struct
-
 import torch
 
 import _mingmoe as _mm
 
 __all__ = ["paged_append", "paged_attn", "paged_attn_workspace", "prompt_attn", "prompt_attn_workspace"]
 
-# mm_pages and mm_batch as bytes, and the current stream by its raw handle: a decode step calls these wrappers once a
-# layer, and building ctypes structures and stream objects took longer than the kernels (a call of
-# paged_append 19.6 -> 11.2 us, of which 4 are the launch)
-_PAGES = struct.Struct("@2P4i8q")
-_BATCH = struct.Struct("@3P4qi4x")
+# The argument blocks as bytes and the current stream by its raw handle: a decode step calls these wrappers once a layer, and
+# building ctypes arguments and stream objects took longer than the kernels (a call of paged_append 19.6 -> 10.8 us, 9.4 where
+# it makes no output; 3.8 of them are the C entry with its launch).
+_APPEND, _PAGED, _PROMPT = (_mm.packer(s) for s in (_mm.PagedAppendArgs, _mm.PagedAttnArgs, _mm.PromptAttnArgs))
 _HALF = (torch.bfloat16, torch.float16)
 _CODES = {torch.bfloat16: _mm.MM_BF16, torch.float16: _mm.MM_FP16, torch.int32: _mm.MM_INT32, torch.int64: _mm.MM_INT64}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
@@ -68,7 +65,7 @@ def _queries(what, q, width, dtype):
 
 
 def _pool(what, k_pages, v_pages):
-    """(mm_pages, n_pages, nkv, page, dqk, dv, dtype) of the pool."""
+    """(mm_pages, nkv, page, dqk, dv, dtype) of the pool."""
     dt = k_pages.dtype
     if k_pages.dim() != 4 or v_pages.dim() != 4 or v_pages.dtype is not dt or dt not in _HALF:
         raise ValueError(f"{what}: k_pages and v_pages must both be bf16 or fp16 [n_pages, nkv, page, d] (got {k_pages.dtype} "
@@ -80,7 +77,7 @@ def _pool(what, k_pages, v_pages):
     if n != m or nkv != vkv or page != vpage or k3 != 1 or v3 != 1:
         raise ValueError(f"{what}: k_pages and v_pages must be [n_pages, nkv, page, d] with one n_pages, nkv and page and "
                          f"contiguous rows (got {list(k_pages.shape)}, {list(v_pages.shape)})")
-    return (_PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), _CODES[dt], nkv, dqk, dv, n, page, k0, k1, k2, v0, v1, v2),
+    return ((k_pages.data_ptr(), v_pages.data_ptr(), _CODES[dt], nkv, dqk, dv, n, page, k0, k1, k2, v0, v1, v2),
             nkv, page, dqk, dv, dt)
 
 
@@ -106,17 +103,20 @@ def _batch(what, page_table, cu_seqlens, kv_lens, tokens):
     if len(shape) != 2 or shape[0] != B or (s[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what}: page_table must be [{B}, pages] with contiguous rows (got {list(shape)}, strides {s})")
     pages = shape[1]
-    return (_BATCH.pack(cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), s[0], pages, B,
-                        tokens, code), B, pages)
+    return ((cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), s[0], pages, B, tokens, code), B, pages)
 
 
-def _call(what, dev, fn, *args):
-    """fn(*args, stream) on device dev's current stream, with dev current."""
+def _on(dev, fn, *args):
+    """fn(*args) with device dev current."""
     if torch.cuda.current_device() == dev:
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _call(what, dev, fn, args):
+    """fn(args, stream) on device dev's current stream."""
+    rc = _on(dev, fn, args, _raw_stream(dev))
     if rc:
         _mm.check(rc, what)
 
@@ -141,7 +141,7 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv
     batch, _, _ = _batch(what, page_table, cu_seqlens, kv_lens, N)
     if not 0 <= rot_offset <= dqk:
         raise ValueError(f"{what}: rot_offset={rot_offset} lies outside a head of {dqk}")
-    inv, pairs = None, 0
+    inv, pairs = 0, 0
     if inv_freq is not None:
         if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
             raise ValueError(f"{what}: inv_freq must be a contiguous fp32 [pairs] tensor (got {inv_freq.dtype} "
@@ -150,9 +150,9 @@ def paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens, inv
     if q_out is None:
         q_out = torch.empty(N, nh, dqk, device=q.device, dtype=dt)
     qo = _rows(what, "q_out", q_out, (N, nh, dqk), dt)
-    ko = (None, 0, 0) if k_out is None else _rows(what, "k_out", k_out, (N, nkv, dqk), dt)
-    _call(what, dev, _mm.load().mm_paged_append, *qr, *kr, *vr, nh, pool, batch, inv, pairs, int(rot_offset),
-          1 if interleaved else 0, *qo, *ko)
+    ko = (0, 0, 0) if k_out is None else _rows(what, "k_out", k_out, (N, nkv, dqk), dt)
+    args = _APPEND.pack(*pool, *batch, *qr, *kr, *vr, *qo, *ko, inv, pairs, nh, int(rot_offset), 1 if interleaved else 0)
+    _call(what, dev, _mm.load().mm_paged_append, args)
     return q_out
 
 
@@ -165,7 +165,7 @@ def _workspace(n, like, workspace):
 
 
 def _bytes(workspace):
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
 def _new_workspace(what, device, size, *args):
@@ -200,8 +200,9 @@ def paged_attn(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, scale=None,
         out = torch.empty(N, nh, dv, device=q.device, dtype=dt)
     o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
-    ws = _workspace(lib.mm_paged_attn_workspace(N, B, pages * page, nh, nkv, dqk, dv, 0), q, workspace)
-    _call(what, dev, lib.mm_paged_attn, *qr, nh, pool, batch, dqk ** -0.5 if scale is None else float(scale), *o, *_bytes(ws))
+    ws = _workspace(_on(dev, lib.mm_paged_attn_workspace, N, B, pages * page, nh, nkv, dqk, dv, 0), q, workspace)
+    args = _PAGED.pack(*pool, *batch, *qr, *o, *_bytes(ws), nh, dqk ** -0.5 if scale is None else scale)
+    _call(what, dev, lib.mm_paged_attn, args)
     return out
 
 
@@ -234,7 +235,8 @@ def prompt_attn(q, k, v, cu_seqlens, scale=None, out=None, workspace=None):
         out = torch.empty(N, nh, dv, device=q.device, dtype=dt)
     o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
-    ws = _workspace(lib.mm_prompt_attn_workspace(N, B, nh, nkv, dqk, dv, 0), q, workspace)
-    _call(what, dev, lib.mm_prompt_attn, *qr, *kr, *vr, _CODES[dt], nh, nkv, dqk, dv, cu_seqlens.data_ptr(), code, B, N,
-          dqk ** -0.5 if scale is None else float(scale), *o, *_bytes(ws))
+    ws = _workspace(_on(dev, lib.mm_prompt_attn_workspace, N, B, nh, nkv, dqk, dv, 0), q, workspace)
+    args = _PROMPT.pack(*qr, *kr, *vr, *o, cu_seqlens.data_ptr(), B, N, *_bytes(ws), code, _CODES[dt], nh, nkv, dqk, dv,
+                        dqk ** -0.5 if scale is None else scale)
+    _call(what, dev, lib.mm_prompt_attn, args)
     return out

@@ -31,7 +31,7 @@ def test_header_declares_the_entry_points_and_the_library_exports_them():
 
 
 # digests of the header's interface (no comments) by version, as tests/test_abi.py keeps them for mingmoe.h
-INTERFACES = {1: "4173de86697e9f74"}
+INTERFACES = {1: "4173de86697e9f74", 2: "d6742157bdb42d72"}
 
 
 def test_the_version_moves_with_the_interface():
@@ -42,7 +42,12 @@ def test_the_version_moves_with_the_interface():
     assert version == mm.PAGED_VERSION == max(INTERFACES)
 
 
-@pytest.mark.parametrize("name,struct", [("mm_pages", mm.Pages), ("mm_batch", mm.Batch)])
+STRUCTS = [("mm_pages", mm.Pages), ("mm_batch", mm.Batch), ("mm_rows", mm.Rows),
+           ("mm_paged_append_args", mm.PagedAppendArgs), ("mm_paged_attn_args", mm.PagedAttnArgs),
+           ("mm_prompt_attn_args", mm.PromptAttnArgs)]
+
+
+@pytest.mark.parametrize("name,struct", STRUCTS)
 def test_struct_layout_matches_c(tmp_path, name, struct):
     src = tmp_path / "layout.c"
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "mingpaged.h"\n'
@@ -52,6 +57,23 @@ def test_struct_layout_matches_c(tmp_path, name, struct):
     subprocess.run(["gcc", "-I", os.path.dirname(HEADER), str(src), "-o", str(exe)], check=True)
     vals = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert vals == [ctypes.sizeof(struct)] + [getattr(struct, f).offset for f, _ in struct._fields_]
+
+
+@pytest.mark.parametrize("name,struct", STRUCTS)
+def test_packed_arguments_lie_as_the_structure_does(name, struct):
+    pack = mm.packer(struct)
+    assert pack.size == ctypes.sizeof(struct)
+
+    def leaves(s, at=0):
+        for f, kind in s._fields_:
+            off = at + getattr(s, f).offset
+            if issubclass(kind, ctypes.Structure):
+                yield from leaves(kind, off)
+            else:
+                yield kind, off
+    places = list(leaves(struct))
+    data = pack.pack(*range(1, len(places) + 1))
+    assert [kind.from_buffer_copy(data, off).value for kind, off in places] == list(range(1, len(places) + 1))
 
 
 # ------------------------------------------------------------------------------------------------ refusals, C entries
@@ -79,19 +101,21 @@ def err(rc):
 
 
 def append(g=None, b=None, q=P, q_ts=512, q_hs=64, k=P, v=P, nh=14, inv=P, pairs=32, off=0, q_out=P, k_out=None):
-    g, b = g or pages(), b or batch()
-    return mm.load().mm_paged_append(q, q_ts, q_hs, k, 128, 64, v, 128, 64, nh, g, b, inv, pairs, off, 0, q_out, 896, 64,
-                                     k_out, 128, 64, None)
+    a = mm.PagedAppendArgs(g or pages(), b or batch(), (q, q_ts, q_hs), (k, 128, 64), (v, 128, 64), (q_out, 896, 64),
+                           (k_out, 128, 64), inv, pairs, nh, off, 0)
+    return mm.load().mm_paged_append(ctypes.byref(a), None)
 
 
 def attn(g=None, b=None, q=P, q_ts=896, nh=14, out=P, o_hs=64, ws=P, ws_bytes=1 << 40):
-    return mm.load().mm_paged_attn(q, q_ts, 64, nh, g or pages(), b or batch(), 0.125, out, 896, o_hs, ws, ws_bytes, None)
+    a = mm.PagedAttnArgs(g or pages(), b or batch(), (q, q_ts, 64), (out, 896, o_hs), ws, ws_bytes, nh, 0.125)
+    return mm.load().mm_paged_attn(ctypes.byref(a), None)
 
 
 def prompt(q=P, k=P, v=P, dtype=mm.MM_BF16, nh=14, nkv=2, dqk=64, dv=64, cu=P, idx=mm.MM_INT32, seqs=3, tokens=5, out=P,
            k_ts=128):
-    return mm.load().mm_prompt_attn(q, 896, 64, k, k_ts, 64, v, 128, 64, dtype, nh, nkv, dqk, dv, cu, idx, seqs, tokens,
-                                    0.125, out, 896, 64, P, 1 << 40, None)
+    a = mm.PromptAttnArgs((q, 896, 64), (k, k_ts, 64), (v, 128, 64), (out, 896, 64), cu, seqs, tokens, P, 1 << 40, idx,
+                          dtype, nh, nkv, dqk, dv, 0.125)
+    return mm.load().mm_prompt_attn(ctypes.byref(a), None)
 
 
 @pytest.mark.parametrize("call", [append, attn])
@@ -116,8 +140,8 @@ def test_append_refuses():
     assert "null q_out" in err(append(q_out=None))
     assert "q must be 16-byte" in err(append(q=P + 2)) and "k_out must be 16-byte" in err(append(k_out=P + 8))
     assert "strides of q" in err(append(q_ts=900)) and "strides of q" in err(append(q_hs=-64))
-    assert "null descriptor" in err(mm.load().mm_paged_append(P, 896, 64, P, 128, 64, P, 128, 64, 14, None, None, P, 32, 0, 0,
-                                                              P, 896, 64, None, 0, 0, None))
+    for entry in (mm.load().mm_paged_append, mm.load().mm_paged_attn, mm.load().mm_prompt_attn):
+        assert "null arguments" in err(entry(None, None))
 
 
 def test_attn_refuses():
