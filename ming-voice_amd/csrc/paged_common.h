@@ -164,9 +164,9 @@ struct AttnArgs {
 
 // How the work is divided. A row is one token's query at one of the G heads that share a key / value head (row r of a
 // stream: token r / G, head r % G), so that a block of BR rows reads each key once for all of them. A stream of n tokens
-// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys may be cut into pieces of `cut` granules of GR keys,
-// one cut for the whole batch, so that a long stream among short ones is shared by many workgroups. cut is at least the sum
-// over all blocks of (granules / target). Only blocks of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there
+// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys may be cut into pieces of up to `cut` granules of GR keys,
+// one cut for the whole batch, so that a long stream among short ones is shared by many workgroups, each block's keys dealt
+// evenly to its pieces. cut is at least the sum over all blocks of (granules / target). Only blocks of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there
 // are at most 2 target of them, a bound that needs no length on the host, as workgroups are at most target + blocks.
 struct Work {
   int b, blk;      // stream (-1: none) and row block
@@ -194,6 +194,17 @@ __device__ __forceinline__ int pieces_of(int keys, int cut) {
   return cut == 0 ? 1 : max(1, (g + cut - 1) / cut);
 }
 
+// The keys begin .. end - 1 of a piece: the block's granules dealt out evenly, so that no piece is a small rest.
+struct Range {
+  int begin, end;
+};
+template <int GR>
+__device__ __forceinline__ Range keys_of_piece(int keys, int pieces, int piece) {
+  const int g = (keys + GR - 1) / GR, each = g / pieces, more = g - each * pieces;
+  const int first = piece * each + min(piece, more);
+  return Range{first * GR, min(keys, (first + each + (piece < more ? 1 : 0)) * GR)};
+}
+
 // Inclusive prefix sums over the wave: within rows of 16 lanes, then rows 0 and 2 into 1 and 3, then lane 31 into the
 // upper half.
 __device__ __forceinline__ int wave_scan(int v) {
@@ -206,19 +217,23 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The granules of a piece: as many pieces as target allows; of many rows (a piece pays for its state of BR rows and the
-// join) kMinCut granules at least.
+// The granules of a piece: as many pieces as target allows, counting half a piece a block for the rounding up of its own
+// number; of many rows (a piece pays for its state of BR rows and the join) kMinCut granules at least.
 constexpr int kMinCut = 4;
 
 template <int BR, int GR, class Load>
 __device__ __forceinline__ int cut_of(const AttnArgs& a, const Stream& mine, Load load) {
   double total = 0.;  // exact in each lane below 2^53
+  float blocks = 0.f;
   for (int base = 0; base < a.batch.seqs; base += kWave) {
     if (base) load(base);
-    total += static_cast<double>(blocks_of<BR>(mine, static_cast<int>(a.group.d))) * ((max(mine.kv, 0) + GR - 1) / GR);
+    const int n = blocks_of<BR>(mine, static_cast<int>(a.group.d));
+    total += static_cast<double>(n) * ((max(mine.kv, 0) + GR - 1) / GR);
+    blocks += static_cast<float>(n);
   }
+  const float target = static_cast<float>(a.target), aim = target - 0.5f * fminf(wave_sum(blocks), target);
   // rounded up by more than the sum over the lanes can lose, so that no cut gives more pieces than target
-  const float cut = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / static_cast<float>(a.target));
+  const float cut = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / aim);
   return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), static_cast<float>((1 << 30) / GR)));
 }
 

@@ -60,8 +60,8 @@ __global__ __launch_bounds__(NW * kWave) void few_kernel(AttnArgs a) {
   }
   const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<P::GR>(keys, w.cut);
   if (w.piece >= pieces) return;
-  const int k_begin = w.piece * w.cut * P::GR;  // one piece: 0
-  const int k_end = w.cut == 0 ? keys : min(keys, k_begin + w.cut * P::GR);
+  const Range part = keys_of_piece<P::GR>(keys, pieces, w.piece);
+  const int k_begin = part.begin, k_end = part.end;
   const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;
   char* kt = s_few + wave * P::WAVE_BYTES;
   char* vt = kt + P::K_BYTES;
@@ -446,7 +446,11 @@ constexpr int64_t kFewReads = 64 << 20;
 int64_t few_granule(int dqk, int dv) { return (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys; }
 // pieces aimed at for one key / value head
 int64_t few_target(int nkv) { return (4 * mm::cu_count() + nkv - 1) / nkv; }
-int64_t many_target(int nkv) { return (2 * mm::cu_count() + nkv - 1) / nkv; }
+// of many rows, as many as the device holds workgroups at once: three a CU by registers at 64 dims, two, or one by shared memory
+int64_t many_target(int nkv, int dqk, int dv) {
+  const int64_t at_once = dqk <= 64 && dv <= 64 ? 3 : dqk <= 192 && dv <= 128 ? 2 : 1;
+  return (at_once * mm::cu_count() + nkv - 1) / nkv;
+}
 int64_t state_bytes(int64_t target, int nkv, int br, int dv) { return 2 * target * nkv * br * (dv + 2) * 4; }
 
 }  // namespace
@@ -458,11 +462,13 @@ int64_t state_bytes(int64_t target, int nkv, int br, int dv) { return 2 * target
 // tokens behind 3000 23.9 | 23.2 (62 MB); 300 tokens of 32/8 heads of 128 16.9 | 13.7 (92 MB); 64 tokens of those behind 8000
 // 66 | 39 (528 MB).
 // Cutting: few rows above 4 granules of keys (one stream at 700 positions: 10.0 us cut, 8.4 not), then 4 pieces a CU (decode of
-// 16 streams behind 4000 to 40000 positions: 397 us uncut, 239 at 1 piece a CU, 217 at 2, 206 at 4, 202 at 8). Many rows over
-// a cache: 2 pieces a CU of at least 4 granules (pieces of 100 to 500 tokens behind 611 to 5000 positions: 149 us uncut, 98
-// at 1, 91 at 2, 101 at 3, 103 at 4; 512 tokens behind 30000: 798 uncut, 414, 316, 386 at 2.5). Prompts, whose keys are
-// their own tokens, only where their row blocks leave half of the CUs idle and can be long (2 heads of 64, 2000 tokens: 24.8
-// us uncut, 15.6 cut; 12 ragged Talker prompts: 42 and 47; 300 tokens of 32/8 heads of 128: 14.0 and 16.5).
+// 16 streams behind 4000 to 40000 positions: 397 us uncut, 239 at 1 piece a CU, 217 at 2, 197 at 4, 202 at 8). Many rows over
+// a cache, above 4 granules: the workgroups that the device holds at once (64 dims, 2000 tokens behind 20000: 280 us at 1.5 a
+// CU, 250 at 3, 242 at 4; 8000 tokens of 2 heads 65 at 1, 50 at 2, 42 at 3, 51 at 4; 128 dims, pieces of 100 to 500 tokens
+// behind 611 to 5000: 149 uncut, 98 at 1, 83 at 2, 97 at 4; 256 dims, 300 tokens behind 5000: 69 at 1, 83 at 2, 600 behind 4000
+// 95 and 106, four times 200 behind 4000 105 and 87). Prompts, whose keys are their own tokens, only where their row blocks
+// leave half of the CUs idle and can be long (2 heads of 64, 2000 tokens: 24.8 us uncut, 15.6 cut; 2000 Talker tokens, 220
+// blocks: 26.6 and 31; 300 tokens of 32/8 heads of 128: 14.0 and 16.5).
 // Two groups of waves to a block where a prompt's blocks are fewer than 4 a CU: they halve the time of the last block (12
 // ragged Talker prompts 42.8 -> 38.5 us, 2000 Talker tokens 37.4 -> 29.6, 4000 72 -> 59), but in a long run two workgroups
 // of one group mix matrix and vector work better (8192 tokens of 32/8 heads of 128: 590 | 643), and over a cache the cut
@@ -473,7 +479,7 @@ AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, i
   p.many = rows > 16 * seqs && reads_of_few(rows, seqs, max_keys, nkv, dqk, dv) > kFewReads;
   p.blocks = most_blocks(rows, seqs, p.many ? 128 : 16);
   if (p.many) {
-    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus && max_keys > 1024) p.target = many_target(nkv);
+    if (paged ? max_keys > 64 * kMinCut : 2 * p.blocks * nkv < cus && max_keys > 1024) p.target = many_target(nkv, dqk, dv);
     p.groups = !paged && p.target == 0 && p.blocks * nkv < 4 * cus && dqk <= 192 && dv <= 128 ? 2 : 1;
     p.workspace = state_bytes(p.target, nkv, 128, dv);
   } else {
@@ -487,7 +493,7 @@ int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys,
   if (!at_most) return plan_attn(paged, tokens, seqs, max_keys, nh, nkv, dqk, dv).workspace;
   const int64_t few = max_keys > 4 * few_granule(dqk, dv) ? state_bytes(few_target(nkv), nkv, 16, dv) : 0;
   const bool many = max_keys > 64 * kMinCut && reads_of_few(tokens * (nh / nkv), seqs, max_keys, nkv, dqk, dv) > kFewReads;
-  const int64_t of_many = many ? state_bytes(many_target(nkv), nkv, 128, dv) : 0;
+  const int64_t of_many = many ? state_bytes(many_target(nkv, dqk, dv), nkv, 128, dv) : 0;
   return few > of_many ? few : of_many;
 }
 

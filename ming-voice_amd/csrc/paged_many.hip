@@ -95,8 +95,8 @@ __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_ker
   }
   const int keys = keys_of<BR>(w.s, w.blk, a.group), pieces = pieces_of<P::GR>(keys, w.cut);
   if (w.piece >= pieces) return;
-  const int k_begin = w.piece * w.cut * P::GR;
-  const int k_end = w.cut == 0 ? keys : min(keys, k_begin + w.cut * P::GR);
+  const Range part = keys_of_piece<P::GR>(keys, pieces, w.piece);
+  const int k_begin = part.begin, k_end = part.end;
   const int tiles = (k_end - k_begin + kKeys - 1) / kKeys;  // group g takes tiles g, g + NG, ..
   const int ctx = w.s.kv - w.s.n;
 

@@ -2,6 +2,7 @@
 arithmetic that turns positions into pages, and the oracle against torch's own attention."""
 import ctypes
 import hashlib
+import math
 import os
 import re
 import subprocess
@@ -318,8 +319,8 @@ def test_oracle_matches_torch_attention():
 # ------------------------------------------------------------------------------------------------ the division of the work
 
 class Division:
-    """The kernels' division of an attention's work (csrc/paged_common.h: stream_at, cut_of, find_work, keys_of, pieces_of),
-    number by number, for blocks of `br` rows and granules of `gr` keys."""
+    """The kernels' division of an attention's work (csrc/paged_common.h: stream_at, cut_of, find_work, keys_of, pieces_of,
+    keys_of_piece), number by number, for blocks of `br` rows and granules of `gr` keys."""
 
     def __init__(self, cu, lens, tokens, group, max_keys, br, gr, target, min_cut):
         self.br, self.gr, self.group, self.target = br, gr, group, target
@@ -331,7 +332,8 @@ class Division:
         self.cut = 0
         if target:
             # the kernel's sum over the lanes is in fp32, rounded up by 1e-5 of it: the least and the most that it can be
-            self.cut = min(max(-(-int(total * 1.00002) // target), min_cut), (1 << 30) // gr)
+            aim = target - min(sum(self.blocks(s) for s in self.streams), target) / 2
+            self.cut = min(max(math.ceil(total * 1.00002 / aim), min_cut), (1 << 30) // gr)
             assert self.cut * target >= total or self.cut == (1 << 30) // gr
 
     def blocks(self, s):
@@ -343,6 +345,12 @@ class Division:
     def keys(self, s, blk):
         last = min(blk * self.br + self.br, s[1] * self.group) - 1
         return 0 if s[2] < 0 else max(0, s[2] - s[1] + last // self.group + 1)
+
+    def part(self, keys, piece):
+        """The keys of a piece."""
+        g, n = -(-keys // self.gr), self.pieces(keys)
+        first = piece * (g // n) + min(piece, g % n)
+        return first * self.gr, min(keys, (first + g // n + (piece < g % n)) * self.gr)
 
     def find(self, w, cut_blocks=False):
         """(stream, block, piece, first slot) of workgroup w, or None."""
@@ -396,7 +404,10 @@ def test_the_work_is_divided_once_and_within_its_bounds(seed):
             done.add((b, blk, piece))
             if pieces > 1:
                 assert 0 <= slot + piece < 2 * target and slots.setdefault(slot + piece, (b, blk, piece)) == (b, blk, piece)
-                assert piece * d.cut * gr < d.keys(s, blk)
+                parts = [d.part(d.keys(s, blk), p) for p in range(pieces)]
+                assert parts[0][0] == 0 and parts[-1][1] == d.keys(s, blk) and all(a < b for a, b in parts)
+                assert all(a[1] == b[0] and a[1] % gr == 0 for a, b in zip(parts, parts[1:]))
+                assert max(b - a for a, b in parts) <= d.cut * gr
         want = {(b, blk, p) for b, s in enumerate(d.streams) for blk in range(d.blocks(s)) for p in range(d.pieces(d.keys(s, blk)))}
         assert done == want
         cut = {(b, blk) for b, blk, p in want if p}
