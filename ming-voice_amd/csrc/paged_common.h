@@ -79,17 +79,24 @@ __device__ __forceinline__ Stream stream_at(const Batch& a, int b) {
   return s;
 }
 
+// How many of the n entries of a rising sequence pass `before`, which the first of them do: 64 probes at a time, by the whole
+// wave (of a sequence that does not rise, some number up to n).
+template <class Before>
+__device__ __forceinline__ int count_before(int n, Before before) {
+  int lo = 0, hi = n;  // the answer lies in lo .. hi
+  while (hi - lo > kWave) {
+    const int step = (hi - lo + kWave - 1) / kWave, i = lo + (lane_id() + 1) * step - 1;
+    const int passed = __popcll(__ballot(i < hi && before(min(i, hi - 1))));
+    lo = min(lo + passed * step, hi);
+    hi = min(lo + step, hi);
+  }
+  const int i = lo + lane_id();
+  return lo + __popcll(__ballot(i < hi && before(min(i, n - 1))));
+}
+
 // The stream that token t belongs to (seqs: none), found by the whole wave: the number of streams that end at or before t.
 __device__ __forceinline__ int stream_of_token(const Batch& a, int t) {
-  int b = 0;
-  for (int base = 0; base < a.seqs; base += kWave) {
-    const int i = base + lane_id();
-    const bool before = i < a.seqs && idx_at(a.cu, a.i64, min(i, a.seqs - 1) + 1) <= t;
-    const int n = __popcll(__ballot(before));
-    b += n;
-    if (n < kWave) break;
-  }
-  return min(b, a.seqs);
+  return count_before(a.seqs, [&](int i) { return idx_at(a.cu, a.i64, i + 1) <= t; });
 }
 
 template <class T>
@@ -160,6 +167,7 @@ struct AttnArgs {
   int negative;
   int target;        // pieces of the keys aimed at, 0: every row block takes all its keys at once
   float* ws;         // the pieces' states
+  int4* index;       // where each stream's work begins (index_kernel), NULL: found anew by each wave
 };
 
 // How the work is divided. A row is one token's query at one of the G heads that share a key / value head (row r of a
@@ -218,23 +226,99 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // The granules of a piece: as many pieces as target allows, counting half a piece a block for the rounding up of its own
-// number; of many rows (a piece pays for its state of BR rows and the join) kMinCut granules at least.
+// number; of many rows (a piece pays for its state of BR rows and the join) kMinCut granules at least. From the batch's
+// granules times blocks, and its blocks.
 constexpr int kMinCut = 4;
+
+template <int BR, int GR>
+__device__ __forceinline__ int cut_for(const AttnArgs& a, float total, float blocks) {
+  const float target = static_cast<float>(a.target), aim = target - 0.5f * fminf(blocks, target);
+  // rounded up by more than the sum over the lanes can lose, so that no cut gives more pieces than target
+  const float cut = ceilf(total * 1.00001f / aim);
+  return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), static_cast<float>((1 << 30) / GR)));
+}
+
+// What a stream adds to the two sums.
+template <int BR, int GR>
+__device__ __forceinline__ void add_stream(const AttnArgs& a, const Stream& s, double& total, float& blocks) {
+  const int n = blocks_of<BR>(s, static_cast<int>(a.group.d));
+  total += static_cast<double>(n) * ((max(s.kv, 0) + GR - 1) / GR);  // exact in each lane below 2^53
+  blocks += static_cast<float>(n);
+}
 
 template <int BR, int GR, class Load>
 __device__ __forceinline__ int cut_of(const AttnArgs& a, const Stream& mine, Load load) {
-  double total = 0.;  // exact in each lane below 2^53
+  double total = 0.;
   float blocks = 0.f;
   for (int base = 0; base < a.batch.seqs; base += kWave) {
     if (base) load(base);
-    const int n = blocks_of<BR>(mine, static_cast<int>(a.group.d));
-    total += static_cast<double>(n) * ((max(mine.kv, 0) + GR - 1) / GR);
-    blocks += static_cast<float>(n);
+    add_stream<BR, GR>(a, mine, total, blocks);
   }
-  const float target = static_cast<float>(a.target), aim = target - 0.5f * fminf(wave_sum(blocks), target);
-  // rounded up by more than the sum over the lanes can lose, so that no cut gives more pieces than target
-  const float cut = ceilf(wave_sum(static_cast<float>(total)) * 1.00001f / aim);
-  return static_cast<int>(fminf(fmaxf(cut, static_cast<float>(BR < 128 ? 1 : kMinCut)), static_cast<float>((1 << 30) / GR)));
+  return cut_for<BR, GR>(a, wave_sum(static_cast<float>(total)), wave_sum(blocks));
+}
+
+// For many streams, what every wave of every workgroup would find by going through them all is written down first: the cut,
+// then behind it for each stream the ends of its workgroups and of its cut blocks among all, and its first state. One
+// workgroup, a stream a thread at a time: bound by the launch and two rounds of reads, 2.0 to 2.6 us at 96 to 256 streams.
+template <int BR, int GR>
+__global__ __launch_bounds__(1024) void index_kernel(AttnArgs a) {
+  constexpr int NW = 1024 / kWave;
+  __shared__ float s_total[NW], s_blocks[NW];
+  __shared__ int s_ends[3][NW];
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, B = a.batch.seqs;
+  int cut = 0;
+  if (a.target > 0) {
+    double total = 0.;
+    float blocks = 0.f;
+    for (int b = tid; b < B; b += 1024) add_stream<BR, GR>(a, stream_at(a.batch, b), total, blocks);
+    const float t = wave_sum(static_cast<float>(total)), n = wave_sum(blocks);
+    if (lane == 0) {
+      s_total[wave] = t;
+      s_blocks[wave] = n;
+    }
+    __syncthreads();
+    float all = 0.f, count = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      all += s_total[x];
+      count += s_blocks[x];
+    }
+    cut = cut_for<BR, GR>(a, all, count);
+  }
+  if (tid == 0) a.index[0] = make_int4(cut, 0, 0, 0);
+  int before[3] = {0, 0, 0};  // of the streams already done: workgroups, cut blocks, states
+  for (int base = 0; base < B; base += 1024) {
+    Stream s{0, 0, 0};
+    if (base + tid < B) s = stream_at(a.batch, base + tid);
+    const int n = blocks_of<BR>(s, static_cast<int>(a.group.d)), p = pieces_of<GR>(max(s.kv, 0), cut);
+    const int mine[3] = {n * p, p > 1 ? n : 0, p > 1 ? n * p : 0};
+    int ends[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ends[i] = wave_scan(mine[i]);
+      if (lane == kWave - 1) s_ends[i][wave] = ends[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ends[i] += before[i];
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        const int v = s_ends[i][x];
+        before[i] += v;
+        if (x < wave) ends[i] += v;
+      }
+    }
+    if (base + tid < B) a.index[base + tid + 1] = make_int4(ends[0], ends[1], ends[2] - mine[2], 0);
+    __syncthreads();  // read before the next round writes
+  }
+}
+
+template <int BR, int GR>
+inline int launch_index(const AttnArgs& a, hipStream_t st, const char* what) {
+  if (!a.index) return MM_OK;
+  hipLaunchKernelGGL((index_kernel<BR, GR>), dim3(1), dim3(1024), 0, st, a);
+  return mm::check_launch(what);
 }
 
 // The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the batch itself: streams 64 at a
@@ -248,6 +332,20 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
     mine = Stream{0, 0, 0};
     if (base + lane < B) mine = stream_at(a.batch, base + lane);
   };
+  if (a.index) {
+    k.cut = a.index[0].x;
+    const int b = count_before(B, [&](int i) { return (CUT ? a.index[i + 1].y : a.index[i + 1].x) <= w; });
+    if (b >= B) return k;
+    const int4 e = a.index[b + 1];
+    k.s = stream_at(a.batch, b);
+    const int nb = blocks_of<BR>(k.s, G), p = pieces_of<GR>(max(k.s.kv, 0), k.cut), units = CUT ? (p > 1 ? nb : 0) : nb * p;
+    const int u = w - ((CUT ? e.y : e.x) - units), at = CUT ? u : u / p;
+    k.blk = nb - 1 - at;
+    k.piece = CUT ? 0 : u - at * p;
+    k.slot = e.z + at * p;
+    if (u >= 0 && u < units && (p == 1 || (k.slot >= 0 && k.slot + p <= 2 * a.target))) k.b = b;
+    return k;
+  }
   load(0);
   if (a.target > 0) {
     k.cut = cut_of<BR, GR>(a, mine, load);
@@ -438,7 +536,7 @@ __device__ __forceinline__ void rows_by_keys(const AttnArgs& a, const Work& w, i
 // at for the whole batch and one key / value head (0: no cutting, no join); blocks: the most row blocks that these sizes
 // can have.
 struct AttnPlan {
-  bool many;
+  bool many, indexed;
   int groups;  // of four waves in a workgroup of many rows
   int64_t blocks, target, workspace;
 };

@@ -424,7 +424,7 @@ int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const cha
   using P = Few<NW, NKQ, NT>;
   auto kern = few_kernel<T, NW, NKQ, NT, PAGED>;
   int rc = mm::allow_lds(kern, P::LDS, what);
-  if (rc) return rc;
+  if (rc || (rc = launch_index<P::BR, P::GR>(a, st, what))) return rc;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)), dim3(NW * kWave), P::LDS, st, a);
   rc = mm::check_launch(what);
   return rc || p.target == 0 ? rc : launch_join<T, P::BR, P::GR, 4, 4>(a, p, st, what);
@@ -450,6 +450,12 @@ int64_t reads_of_few(int64_t rows, int64_t seqs, int64_t max_keys, int nkv, int 
 }
 constexpr int64_t kFewReads = 64 << 20;
 
+// Streams up to which every wave finds its work by itself, 64 of them at a time; of more, index_kernel writes down where each
+// stream's begins. us a call without | with it: one token of 192 Talker streams behind 1500 positions 54 | 46, behind 200 10.0 |
+// 12.3; 8 tokens each behind 300 38 | 29; of 128 streams 35 | 34, 8.0 | 10.6, 25 | 25; of 1024 311 | 155, 65 | 39; of 4096 behind
+// 200 601 | 134; 2048 prompts of 20 tokens 173 | 100, 192 of them 22.3 | 22.6.
+constexpr int64_t kIndexed = 128;
+
 int64_t few_granule(int dqk, int dv) { return (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys; }
 // pieces aimed at for one key / value head
 int64_t few_target(int nkv) { return (4 * mm::cu_count() + nkv - 1) / nkv; }
@@ -458,6 +464,7 @@ int64_t many_target(int nkv, int dqk, int dv) {
   const int64_t at_once = dqk <= 64 && dv <= 64 ? 3 : dqk <= 192 && dv <= 128 ? 2 : 1;
   return (at_once * mm::cu_count() + nkv - 1) / nkv;
 }
+int64_t index_bytes(int64_t seqs) { return seqs > kIndexed ? 16 * (seqs + 1) : 0; }
 int64_t state_bytes(int64_t target, int nkv, int br, int dv) { return 2 * target * nkv * br * (dv + 2) * 4; }
 
 }  // namespace
@@ -493,6 +500,8 @@ AttnPlan plan_attn(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys, i
     if (max_keys > 4 * few_granule(dqk, dv)) p.target = few_target(nkv);
     p.workspace = state_bytes(p.target, nkv, 16, dv);
   }
+  p.indexed = seqs > kIndexed;
+  p.workspace += index_bytes(seqs);
   return p;
 }
 
@@ -501,7 +510,7 @@ int64_t workspace_of(bool paged, int64_t tokens, int64_t seqs, int64_t max_keys,
   const int64_t few = max_keys > 4 * few_granule(dqk, dv) ? state_bytes(few_target(nkv), nkv, 16, dv) : 0;
   const bool many = max_keys > 64 * kMinCut && reads_of_few(tokens * (nh / nkv), seqs, max_keys, nkv, dqk, dv) > kFewReads;
   const int64_t of_many = many ? state_bytes(many_target(nkv, dqk, dv), nkv, 128, dv) : 0;
-  return few > of_many ? few : of_many;
+  return (few > of_many ? few : of_many) + index_bytes(seqs);
 }
 
 int launch_few(const AttnArgs& a, const AttnPlan& p, int dtype, bool paged, hipStream_t st, const char* what) {

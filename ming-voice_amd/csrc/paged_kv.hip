@@ -243,7 +243,8 @@ int attend(AttnArgs& a, int dtype, bool paged, float scale, void* workspace, int
   MM_REQUIRE((p.blocks + p.target) * a.nkv < (1LL << 23), "%s: too many streams and rows for one launch", what);
   MM_REQUIRE(p.workspace == 0 || (workspace && mm::aligned16(workspace) && workspace_bytes >= p.workspace),
              "%s: a 16-byte aligned workspace of %lld bytes is needed", what, (long long)p.workspace);
-  a.ws = static_cast<float*>(workspace);
+  a.index = p.indexed ? static_cast<int4*>(workspace) : nullptr;
+  a.ws = static_cast<float*>(workspace) + (p.indexed ? 4 * (a.batch.seqs + static_cast<int64_t>(1)) : 0);
   a.target = static_cast<int>(p.target);
   return p.many ? launch_many(a, p, dtype, paged, st, what) : launch_few(a, p, dtype, paged, st, what);
 }

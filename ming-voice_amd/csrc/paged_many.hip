@@ -412,6 +412,9 @@ __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_ker
 
 template <class T, int KS, int VS, int NG, int SRC>
 int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const char* what) {
+  using P = Many<KS, VS, NG>;
+  int rc = launch_index<P::BR, P::GR>(a, st, what);
+  if (rc) return rc;
   hipLaunchKernelGGL((many_kernel<T, KS, VS, NG, SRC>), dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)),
                      dim3(NG * kWaves * kWave), 0, st, a);
   return mm::check_launch(what);

@@ -196,7 +196,7 @@ def test_long_contexts(nh, nkv, dqk, dv, new, ctx):
     assert torch.equal(first, s.attn())  # sums are joined in one order
 
 
-@pytest.mark.parametrize("count", [63, 64, 65, 130, 700])
+@pytest.mark.parametrize("count", [63, 64, 65, 128, 129, 700, 1100, 4200])
 @BOTH
 def test_many_streams(count, kind):
     new = [(0, 1, 30)[i % 3] if kind == "many" else i % 3 for i in range(count)]
@@ -464,6 +464,37 @@ def test_one_graph_serves_every_length(idx):
         check(got[:n], O.paged_attn(want_q[:n], eager.kp, eager.vp, s.table, s.cu, s.lens, 64 ** -0.5), 2600, 64, BF)
 
 
+@BOTH
+def test_one_graph_serves_every_length_of_many_streams(kind):
+    """The same with an index of the streams (more than 128), in one captured call and its workspace."""
+    B = 200
+    cases = [Streams([(1, 0, 3)[(i * k) % 3] if i < n else 0 for i in range(B)], [(i * k * 61) % 900 for i in range(B)],
+                     4, 2, 64, 64, seed=70 + k, spare=600, more_pages=many_pages(kind, 16)) for k, n in ((1, 200), (2, 130), (5, 1))]
+    rows = max(len(s.q) for s in cases)
+    q = torch.zeros(rows, 4, 64, device=DEV, dtype=BF)
+    out = torch.zeros(rows, 4, 64, device=DEV, dtype=BF)
+    kp, vp = (torch.zeros(max(s.kp.shape[0] for s in cases), 2, 16, 64, device=DEV, dtype=BF) for _ in range(2))
+    table = torch.zeros(B, max(s.table.shape[1] for s in cases), device=DEV, dtype=torch.int32)
+    cu, lens = (torch.zeros(n, device=DEV, dtype=torch.int32) for n in (B + 1, B))
+    ws = PK.paged_attn_workspace(rows, B, table.shape[1] * 16, 4, 2, 64, 64)
+    graph = torch.cuda.CUDAGraph()
+    PK.paged_attn(q, kp, vp, table, cu, lens, out=out, workspace=ws)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        PK.paged_attn(q, kp, vp, table, cu, lens, out=out, workspace=ws)
+    for s in cases + cases[::-1]:
+        table.fill_(-1)
+        for dst, src in ((q[:len(s.q)], s.q), (cu, s.cu), (lens, s.lens), (table[:, :s.table.shape[1]], s.table),
+                         (kp[:s.kp.shape[0]], s.kp), (vp[:s.vp.shape[0]], s.vp)):
+            dst.copy_(src)
+        out.fill_(5.0)
+        ws.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[s.N:] == 5.0).all()
+        check(out[:s.N], s.oracle(), 1000, 64, BF)
+
+
 def test_another_stream_and_a_shared_workspace():
     s = Streams([1, 1, 5], [6000, 20, 300], seed=71)
     want = s.attn()
@@ -529,6 +560,19 @@ def test_indices_that_make_no_sense_stay_in_bounds(kind):
     s = Streams([5, 60, 3], [100, 900, 0], seed=83, more_pages=many_pages(kind, 16))
     for cu in ([0, 65, 5, 68], [3, 5, 65, 68], [0, 5, 65, 9999], [-7, 5, 65, 68], [68, 0, 68, 0], [0, 68, 0, 68]):
         s.cu = torch.tensor(cu, device=DEV, dtype=torch.int32)
+        s.attn()
+        PK.prompt_attn(s.q, s.k, s.v, s.cu)
+        PK.paged_append(s.q, s.k, s.v, s.kp, s.vp, s.table, s.cu, s.lens)
+        torch.cuda.synchronize()
+
+
+@BOTH
+def test_indices_of_many_streams_that_make_no_sense_stay_in_bounds(kind):
+    """The same where the streams are indexed first."""
+    s = Streams([1] * 150, [(i * 7) % 300 for i in range(150)], seed=84, spare=40, more_pages=many_pages(kind, 16))
+    up = torch.arange(151, device=DEV, dtype=torch.int32)
+    for cu in (up.flip(0), (up * 73) % 160, up * 5 - 200, torch.where(up % 2 == 0, 0, 190).int()):
+        s.cu = cu.contiguous()
         s.attn()
         PK.prompt_attn(s.q, s.k, s.v, s.cu)
         PK.paged_append(s.q, s.k, s.v, s.kp, s.vp, s.table, s.cu, s.lens)

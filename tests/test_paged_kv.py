@@ -370,6 +370,53 @@ class Division:
         return None
 
 
+    def index(self):
+        """index_kernel: for each stream the ends of its workgroups and of its cut blocks, and its first state."""
+        units = cut = held = 0
+        for s in self.streams:
+            nb, p = self.blocks(s), self.pieces(max(s[2], 0))
+            units, cut, first = units + nb * p, cut + (nb if p > 1 else 0), held
+            held += nb * p if p > 1 else 0
+            yield units, cut, first
+
+    def find_indexed(self, w, index, cut_blocks=False):
+        """find by the index, as the kernels do it for many streams."""
+        ends = [e[1 if cut_blocks else 0] for e in index]
+        b = count_before(len(ends), lambda i: ends[i] <= w)
+        if b >= len(ends):
+            return None
+        s, nb, p = self.streams[b], self.blocks(self.streams[b]), self.pieces(max(self.streams[b][2], 0))
+        units = (nb if p > 1 else 0) if cut_blocks else nb * p
+        u = w - (ends[b] - units)
+        at = u if cut_blocks else u // max(p, 1)
+        slot = index[b][2] + at * p
+        if not 0 <= u < units or (p > 1 and not 0 <= slot <= 2 * self.target - p):
+            return None
+        return b, nb - 1 - at, 0 if cut_blocks else u - at * p, slot
+
+
+def count_before(n, before):
+    """The kernels' search (csrc/paged_common.h: count_before): every probe stays inside the sequence."""
+    def probe(i):
+        assert 0 <= i < n
+        return before(i)
+    lo, hi = 0, n
+    while hi - lo > 64:
+        step = -(-(hi - lo) // 64)
+        at = [lo + (lane + 1) * step - 1 for lane in range(64)]
+        passed = sum(probe(min(i, hi - 1)) and i < hi for i in at)
+        lo = min(lo + passed * step, hi)
+        hi = min(lo + step, hi)
+    return lo + sum(probe(min(lo + lane, n - 1)) and lo + lane < hi for lane in range(64))
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 127, 128, 129, 4096, 4097, 4225, 100000])
+def test_the_search_counts_what_comes_before(n):
+    for answer in {0, 1, 2, 62, 63, 64, 65, 66, n // 2, n - 65, n - 64, n - 63, n - 1, n} & set(range(n + 1)):
+        assert count_before(n, lambda i: i < answer) == answer
+    assert 0 <= count_before(n, lambda i: i % 3 == 1) <= n  # nonsense stays in bounds
+
+
 def _divisions(seed):
     import random
     r = random.Random(seed)
@@ -390,9 +437,11 @@ def test_the_work_is_divided_once_and_within_its_bounds(seed):
         rows = N * group
         blocks = min(rows // br + len(new), rows)
         grid = blocks + target  # what the host launches for these sizes
-        done, slots = set(), {}
+        done, slots, index = set(), {}, list(d.index())
         for w in range(grid):
             f = d.find(w)
+            if w % 5 == 0 or w < 70:
+                assert d.find_indexed(w, index) == f and d.find_indexed(w, index, True) == d.find(w, True)
             if f is None:
                 continue
             b, blk, piece, slot = f
@@ -422,9 +471,9 @@ def test_the_work_is_divided_once_and_within_its_bounds(seed):
 def test_a_division_of_nonsense_stays_in_bounds(cu, br, gr, min_cut, target):
     N, group, lens, most = 68, 7, [105, 960, 3], 970
     d = Division(cu, lens, N, group, most, br, gr, target, min_cut)
+    index = list(d.index())
     for w in range(min(N * group // br + 3, N * group) + target):
-        for cut_blocks in (False, True):
-            f = d.find(w, cut_blocks)
+        for f in (d.find(w), d.find(w, True), d.find_indexed(w, index), d.find_indexed(w, index, True)):
             if f is None:
                 continue
             b, blk, piece, slot = f
