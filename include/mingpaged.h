@@ -101,7 +101,8 @@ int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t max_keys, 
  * get NaN. Rows past a token's position never reach it, whatever they hold. out must not overlap q or the pool. workspace:
  * mm_paged_attn_workspace bytes, 16-byte aligned (NULL where that is 0), no initialisation; calls that share one must not
  * overlap in time. Equal calls give equal bits; the order of a token's sums depends on the whole batch's lengths. Limits:
- * tokens 2^22, tokens * nh 2^30, streams 2^20, max_pages * page 2^30. */
+ * tokens 2^22, tokens * nh 2^30, streams 2^20, max_pages * page 2^30; a launch of 2^23 workgroups (blocks of 16 or 128 rows
+ * times key / value heads, a stream's own each) is refused. */
 typedef struct mm_paged_attn_args {
   mm_pages pages;
   mm_batch batch;

@@ -172,10 +172,11 @@ struct AttnArgs {
 
 // How the work is divided. A row is one token's query at one of the G heads that share a key / value head (row r of a
 // stream: token r / G, head r % G), so that a block of BR rows reads each key once for all of them. A stream of n tokens
-// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys may be cut into pieces of up to `cut` granules of GR keys,
-// one cut for the whole batch, so that a long stream among short ones is shared by many workgroups, each block's keys dealt
-// evenly to its pieces. cut is at least the sum over all blocks of (granules / target). Only blocks of more than one piece keep states: ceil(x) <= 2 x for x > 1, so there
-// are at most 2 target of them, a bound that needs no length on the host, as workgroups are at most target + blocks.
+// has ceil(n G / BR) row blocks, and where `target` > 0 a block's keys may be cut into pieces of up to `cut` granules of GR
+// keys, one cut for the whole batch, so that a long stream among short ones is shared by many workgroups, each block's keys
+// dealt evenly to its pieces. cut is at least the sum over all blocks of (granules / target). Only blocks of more than one
+// piece keep states: ceil(x) <= 2 x for x > 1, so there are at most 2 target of them, a bound that needs no length on the
+// host, as workgroups are at most target + blocks.
 struct Work {
   int b, blk;      // stream (-1: none) and row block
   int piece;       // of the block's keys
@@ -321,8 +322,9 @@ inline int launch_index(const AttnArgs& a, hipStream_t st, const char* what) {
   return mm::check_launch(what);
 }
 
-// The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the batch itself: streams 64 at a
-// time, one to a lane. Within a stream the last row block, whose rows see the most keys, comes first.
+// The work of workgroup w (CUT: row block w of those that are cut, at most target of them), found by every wave from the
+// batch itself, streams 64 at a time, one to a lane, or from the index. Within a stream the last row block, whose rows see
+// the most keys, comes first.
 template <int BR, int GR, bool CUT>
 __device__ __forceinline__ Work find_work(const AttnArgs& a, int w) {
   const int G = static_cast<int>(a.group.d), lane = lane_id(), B = a.batch.seqs;

@@ -360,8 +360,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 }
 
 // The same for blocks of many rows, which are cut into few pieces: dv / 4 lanes to a row, each through all pieces. Grid (cut
-// blocks, key / value heads, BR / ROWS) x 256. Bound by latency too: 8 us after pieces of 100 to 500 tokens of 32/8 heads behind
-// 611 to 5000 positions (79 us).
+// blocks, key / value heads, BR / ROWS) x 256. Bound by latency too: 8 us after pieces of 100 to 500 tokens of 32/8 heads
+// behind 611 to 5000 positions (79 us).
 template <class T, int BR, int GR, int ROWS>
 __global__ __launch_bounds__(256) void join_rows_kernel(AttnArgs a) {
   const int tid = threadIdx.x, kvh = blockIdx.y, G = static_cast<int>(a.group.d);
@@ -459,7 +459,8 @@ constexpr int64_t kIndexed = 128;
 int64_t few_granule(int dqk, int dv) { return (dqk <= 192 && dv <= 128 ? 8 : 4) * kKeys; }
 // pieces aimed at for one key / value head
 int64_t few_target(int nkv) { return (4 * mm::cu_count() + nkv - 1) / nkv; }
-// of many rows, as many as the device holds workgroups at once: three a CU by registers at 64 dims, two, or one by shared memory
+// of many rows, as many as the device holds workgroups at once: three a CU by registers at 64 dims, two, or one by shared
+// memory
 int64_t many_target(int nkv, int dqk, int dv) {
   const int64_t at_once = dqk <= 64 && dv <= 64 ? 3 : dqk <= 192 && dv <= 128 ? 2 : 1;
   return (at_once * mm::cu_count() + nkv - 1) / nkv;

@@ -174,13 +174,15 @@ constexpr int64_t kMaxTokens = 1 << 22, kMaxSeqs = 1 << 20, kMaxPages = (1LL << 
 // positions of a stream, and rows (tokens times heads): 32-bit numbers of them stay positive with a tile or a piece added
 constexpr int64_t kMaxKeys = 1LL << 30, kMaxRows = 1LL << 30;
 
-int check_rows(const char* what, const char* name, const mm_rows& r, int64_t tokens, int heads, int align) {
+// Rows that are written must not lie on each other: no stride of zero.
+int check_rows(const char* what, const char* name, const mm_rows& r, int64_t tokens, int heads, int align, bool written = false) {
   const int64_t ts = r.token_stride, hs = r.head_stride;
   MM_REQUIRE(r.p, "%s: null %s", what, name);
   MM_REQUIRE((reinterpret_cast<uintptr_t>(r.p) & static_cast<uintptr_t>(align - 1)) == 0, "%s: %s must be %d-byte aligned",
              what, name, align);
   MM_REQUIRE((tokens == 1 || (ts >= 0 && ts % (align / 2) == 0)) && (heads == 1 || (hs >= 0 && hs % (align / 2) == 0)),
              "%s: strides of %s must keep rows %d-byte aligned", what, name, align);
+  MM_REQUIRE(!written || ((tokens == 1 || ts > 0) && (heads == 1 || hs > 0)), "%s: rows of %s lie on each other", what, name);
   return MM_OK;
 }
 
@@ -199,7 +201,7 @@ int check_tokens(const char* what, int64_t tokens, int64_t seqs) {
   return MM_OK;
 }
 
-int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) {
+int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b, bool written) {
   int rc = check_shape(what, g->dtype, nh, g->nkv, g->dqk, g->dv);
   if (rc) return rc;
   if ((rc = check_tokens(what, b->tokens, b->seqs))) return rc;
@@ -213,7 +215,8 @@ int check_paged(const char* what, int nh, const mm_pages* g, const mm_batch* b) 
   const int64_t st[6] = {g->k_page_stride, g->k_head_stride, g->k_row_stride, g->v_page_stride, g->v_head_stride, g->v_row_stride};
   const int64_t dims[3] = {g->n_pages, g->nkv, g->page};
   for (int i = 0; i < 6; ++i)
-    MM_REQUIRE(dims[i % 3] <= 1 || (st[i] >= 0 && st[i] % 8 == 0), "%s: the pool's strides must be multiples of 8", what);
+    MM_REQUIRE(dims[i % 3] <= 1 || (st[i] >= (written ? 8 : 0) && st[i] % 8 == 0),
+               written ? "%s: the pool's strides must be multiples of 8, not 0" : "%s: the pool's strides must be multiples of 8", what);
   return MM_OK;
 }
 
@@ -256,7 +259,7 @@ extern "C" int mm_paged_version(void) { return MM_PAGED_VERSION; }
 extern "C" int mm_paged_append(const mm_paged_append_args* g, void* stream) {
   const char* what = "paged_append";
   MM_REQUIRE(g, "%s: null arguments", what);
-  int rc = check_paged(what, g->nh, &g->pages, &g->batch);
+  int rc = check_paged(what, g->nh, &g->pages, &g->batch, true);
   if (rc) return rc;
   const int64_t pairs = g->inv_freq ? g->pairs : 0;
   const int rot_offset = g->inv_freq ? g->rot_offset : 0, nkv = g->pages.nkv;
@@ -267,9 +270,9 @@ extern "C" int mm_paged_append(const mm_paged_append_args* g, void* stream) {
   const int64_t N = g->batch.tokens;
   if (N == 0 || g->batch.seqs == 0) return MM_OK;
   if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "k", g->k, N, nkv, 16)) ||
-      (rc = check_rows(what, "v", g->v, N, nkv, 16)) || (rc = check_rows(what, "q_out", g->q_out, N, g->nh, 16)))
+      (rc = check_rows(what, "v", g->v, N, nkv, 16)) || (rc = check_rows(what, "q_out", g->q_out, N, g->nh, 16, true)))
     return rc;
-  if (g->k_out.p && (rc = check_rows(what, "k_out", g->k_out, N, nkv, 16))) return rc;
+  if (g->k_out.p && (rc = check_rows(what, "k_out", g->k_out, N, nkv, 16, true))) return rc;
   AppendArgs a{};
   a.q = rows_of(g->q);
   a.k = rows_of(g->k);
@@ -307,11 +310,11 @@ extern "C" int64_t mm_paged_attn_workspace(int64_t tokens, int64_t seqs, int64_t
 extern "C" int mm_paged_attn(const mm_paged_attn_args* g, void* stream) {
   const char* what = "paged_attn";
   MM_REQUIRE(g, "%s: null arguments", what);
-  int rc = check_paged(what, g->nh, &g->pages, &g->batch);
+  int rc = check_paged(what, g->nh, &g->pages, &g->batch, false);
   if (rc) return rc;
   const int64_t N = g->batch.tokens;
   if (N == 0 || g->batch.seqs == 0) return MM_OK;
-  if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8))) return rc;
+  if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8, true))) return rc;
   AttnArgs a{};
   a.q = rows_of(g->q);
   a.out = rows_of(g->out);
@@ -344,7 +347,7 @@ extern "C" int mm_prompt_attn(const mm_prompt_attn_args* g, void* stream) {
   MM_REQUIRE(N * g->nh <= kMaxRows, "%s: tokens * nh must be at most 2^30", what);
   if (N == 0 || g->seqs == 0) return MM_OK;
   if ((rc = check_rows(what, "q", g->q, N, g->nh, 16)) || (rc = check_rows(what, "k", g->k, N, g->nkv, 16)) ||
-      (rc = check_rows(what, "v", g->v, N, g->nkv, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8)))
+      (rc = check_rows(what, "v", g->v, N, g->nkv, 16)) || (rc = check_rows(what, "out", g->out, N, g->nh, 8, true)))
     return rc;
   AttnArgs a{};
   a.q = rows_of(g->q);

@@ -164,8 +164,12 @@ def _workspace(n, like, workspace):
     return workspace
 
 
-def _bytes(workspace):
-    return (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+def _bytes(what, workspace):
+    if workspace is None:
+        return 0, 0
+    if not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous (got {list(workspace.shape)}, strides {workspace.stride()})")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _new_workspace(what, device, size, *args):
@@ -201,7 +205,7 @@ def paged_attn(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, scale=None,
     o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
     ws = _workspace(_on(dev, lib.mm_paged_attn_workspace, N, B, pages * page, nh, nkv, dqk, dv, 0), q, workspace)
-    args = _PAGED.pack(*pool, *batch, *qr, *o, *_bytes(ws), nh, dqk ** -0.5 if scale is None else scale)
+    args = _PAGED.pack(*pool, *batch, *qr, *o, *_bytes(what, ws), nh, dqk ** -0.5 if scale is None else scale)
     _call(what, dev, lib.mm_paged_attn, args)
     return out
 
@@ -236,7 +240,7 @@ def prompt_attn(q, k, v, cu_seqlens, scale=None, out=None, workspace=None):
     o = _rows(what, "out", out, (N, nh, dv), dt)
     lib = _mm.load()
     ws = _workspace(_on(dev, lib.mm_prompt_attn_workspace, N, B, nh, nkv, dqk, dv, 0), q, workspace)
-    args = _PROMPT.pack(*qr, *kr, *vr, *o, cu_seqlens.data_ptr(), B, N, *_bytes(ws), code, _CODES[dt], nh, nkv, dqk, dv,
+    args = _PROMPT.pack(*qr, *kr, *vr, *o, cu_seqlens.data_ptr(), B, N, *_bytes(what, ws), code, _CODES[dt], nh, nkv, dqk, dv,
                         dqk ** -0.5 if scale is None else scale)
     _call(what, dev, lib.mm_prompt_attn, args)
     return out

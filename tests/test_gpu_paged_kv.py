@@ -376,6 +376,31 @@ def test_broadcast_and_strided_inputs():
     assert torch.equal(PK.prompt_attn(heads_first, k, v, s.cu, out=out), want)
 
 
+@BOTH
+def test_streams_that_share_their_first_pages(kind):
+    """A common prompt's pages in three streams' tables, one of them only partly filled by it."""
+    s = Streams([1, 30, 2], [64, 40, 200], seed=45, more_pages=many_pages(kind, 16))
+    s.table[1, :2] = s.table[0, :2]
+    s.table[2, :4] = s.table[0, :4]
+    check(s.attn(), s.oracle(), 250, 64, BF)
+
+
+@BOTH
+def test_rows_before_the_first_stream_are_left_as_they_were(kind):
+    s = Streams([3, 40, 1], [9, 100, 700], seed=46, more_pages=many_pages(kind, 16))
+    wide = torch.cat([torch.full((5, *s.q.shape[1:]), float("nan"), device=DEV, dtype=BF), s.q])
+    out = torch.full((5 + s.N, s.nh, s.dv), 9.0, device=DEV, dtype=BF)
+    PK.paged_attn(wide, s.kp, s.vp, s.table, s.cu + 5, s.lens, out=out)
+    assert (out[:5] == 9.0).all()
+    check(out[5:], s.oracle(), 800, 64, BF)
+    q = torch.full_like(wide, 9.0)
+    k, v = (torch.cat([t[:1].expand(5, -1, -1), t]) for t in (s.k, s.v))
+    kp = s.kp.clone()
+    PK.paged_append(wide, k, v, s.kp, s.vp, s.table, s.cu + 5, s.lens, q_out=q)
+    assert (q[:5] == 9.0).all() and torch.equal(q[5:], s.q)
+    assert int((s.kp.nan_to_num(7.0) != kp.nan_to_num(7.0)).any(-1).any(1).sum()) <= s.N
+
+
 def test_a_contiguous_cache_is_one_page():
     """A stream's static cache [nkv, max_len, hd] is a pool of one page."""
     s = Streams([1], [200], page=256, seed=47, more_pages=0)

@@ -101,8 +101,9 @@ def err(rc):
     return mm.last_error()
 
 
-def append(g=None, b=None, q=P, q_ts=512, q_hs=64, k=P, v=P, nh=14, inv=P, pairs=32, off=0, q_out=P, k_out=None):
-    a = mm.PagedAppendArgs(g or pages(), b or batch(), (q, q_ts, q_hs), (k, 128, 64), (v, 128, 64), (q_out, 896, 64),
+def append(g=None, b=None, q=P, q_ts=512, q_hs=64, k=P, v=P, nh=14, inv=P, pairs=32, off=0, q_out=P, k_out=None,
+           qo_ts=896):
+    a = mm.PagedAppendArgs(g or pages(), b or batch(), (q, q_ts, q_hs), (k, 128, 64), (v, 128, 64), (q_out, qo_ts, 64),
                            (k_out, 128, 64), inv, pairs, nh, off, 0)
     return mm.load().mm_paged_append(ctypes.byref(a), None)
 
@@ -140,6 +141,7 @@ def test_append_refuses():
     assert "null q" in err(append(q=None)) and "null k" in err(append(k=None)) and "null v" in err(append(v=None))
     assert "null q_out" in err(append(q_out=None))
     assert "q must be 16-byte" in err(append(q=P + 2)) and "k_out must be 16-byte" in err(append(k_out=P + 8))
+    assert "on each other" in err(append(g=pages(), q_out=P, qo_ts=0)) and "strides must be" in err(append(g=pages(k_row_stride=0)))
     assert "strides of q" in err(append(q_ts=900)) and "strides of q" in err(append(q_hs=-64))
     for entry in (mm.load().mm_paged_append, mm.load().mm_paged_attn, mm.load().mm_prompt_attn):
         assert "null arguments" in err(entry(None, None))
@@ -148,7 +150,7 @@ def test_append_refuses():
 def test_attn_refuses():
     assert "null q" in err(attn(q=None)) and "null out" in err(attn(out=None))
     assert "strides of q" in err(attn(q_ts=892)) and "out must be 8-byte" in err(attn(out=P + 4))
-    assert "strides of out" in err(attn(o_hs=66))
+    assert "strides of out" in err(attn(o_hs=66)) and "on each other" in err(attn(o_hs=0))
     assert "tokens * nh" in err(attn(b=batch(tokens=1 << 22), nh=512))
     need = mm.load().mm_paged_attn_workspace(5, 3, 16 * 1000, 14, 2, 64, 64, 0)  # a table that allows long contexts
     long = batch(max_pages=1000, table_stride=1000)
@@ -223,6 +225,7 @@ def test_wrappers_take_gpu_tensors_only():
 def any_device(monkeypatch):
     """The wrappers' own checks on CPU tensors: none of the refused calls reaches the library."""
     monkeypatch.setattr(mm, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(PK, "_on", lambda dev, fn, *a: fn(*a))
     monkeypatch.setattr(PK, "_call", lambda *a: pytest.fail("the call was not refused"))
 
 
@@ -259,7 +262,8 @@ def test_append_wrapper_refuses(any_device, what, change):
     ("q must be", dict(q=torch.zeros(3, 4, 24, dtype=BF))), ("q must be", dict(q=torch.zeros(3, 4, 16, dtype=torch.float16))),
     ("k_pages and v_pages must be", dict(v_pages=torch.zeros(4, 2, 4, 8, dtype=BF))),
     ("out must be", dict(out=torch.zeros(2, 4, 8, dtype=BF))), ("out must be", dict(out=torch.zeros(3, 4, 16, dtype=BF))),
-    ("one dtype", dict(page_table=torch.zeros(2, 3, dtype=torch.int64)))])
+    ("one dtype", dict(page_table=torch.zeros(2, 3, dtype=torch.int64))),
+    ("workspace must be contiguous", dict(workspace=torch.zeros(1).expand(1 << 20)))])
 def test_attn_wrapper_refuses(any_device, what, change):
     a = {k: v for k, v in _args().items() if k not in "kv"}
     with pytest.raises(ValueError, match=what):
@@ -271,7 +275,8 @@ def test_attn_wrapper_refuses(any_device, what, change):
     ("k must be", dict(k=torch.zeros(4, 2, 16, dtype=BF))),
     ("v must be", dict(v=torch.zeros(3, 1, 8, dtype=BF))), ("v must be", dict(v=torch.zeros(2, 2, 8, dtype=BF))), ("q, k and v must be", dict(v=torch.zeros(3, 16, dtype=BF))),
     ("cu_seqlens", dict(cu_seqlens=torch.zeros(2, 2, dtype=torch.int32))),
-    ("out must be", dict(out=torch.zeros(3, 4, 8)))])
+    ("out must be", dict(out=torch.zeros(3, 4, 8))),
+    ("workspace must be contiguous", dict(workspace=torch.zeros(1 << 10)[::2]))])
 def test_prompt_wrapper_refuses(any_device, what, change):
     a = {k: v for k, v in _args().items() if k in ("q", "k", "v", "cu_seqlens")}
     with pytest.raises(ValueError, match=what):
