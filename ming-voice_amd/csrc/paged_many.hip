@@ -117,17 +117,27 @@ __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_ker
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * r, static_cast<int>(v >> 32)));
     return reinterpret_cast<const char*>((static_cast<uint64_t>(hi) << 32) | lo);
   };
-  // the page numbers of a tile: of key l (kAnywhere), of keys 8 (l % 8) .. + 7 (kPaged)
+  // the page numbers of a tile: of key l (kAnywhere), of keys 8 (l % 8) .. + 7 (kPaged; pages of 8 rows or more, so that the
+  // offset in a table's row fits 32 bits and the divisor is not 1)
+  auto page_of = [&](int key) { return __umulhi(static_cast<uint32_t>(key), a.page.m) >> a.page.s; };
+  const char* pages = SRC == kPaged ? static_cast<const char*>(a.batch.table) + w.b * a.batch.table_stride * (a.batch.i64 ? 8 : 4) : nullptr;
   auto ids_of = [&](int it) {
-    const int key = k_begin + it * kKeys + (SRC == kAnywhere ? lane : 8 * (lane % 8));
+    const int key = min(k_begin + it * kKeys + (SRC == kAnywhere ? lane : 8 * (lane % 8)), k_end - 1);
     if (SRC == kPacked || (SRC == kAnywhere && !a.batch.table)) return Index{0, 0};
-    return page_id(a, w.b, min(key, k_end - 1));
+    if (SRC == kAnywhere) return page_id(a, w.b, key);
+    const auto* at = reinterpret_cast<const uint32_t*>(pages + (page_of(key) << (a.batch.i64 ? 3 : 2)));
+    Index id{at[0], 0};
+    if (a.batch.i64) id.hi = at[1];
+    return id;
   };
   const char *kpk = nullptr, *vpk = nullptr;  // kPacked: the wave's first row of the tile to load
   if constexpr (SRC == kPacked) {
     kpk = reinterpret_cast<const char*>(a.k.at(w.s.first + k_begin + kKeys * group + 8 * wave, kvh));
     vpk = reinterpret_cast<const char*>(a.v.at(w.s.first + k_begin + kKeys * group + 8 * wave, kvh));
   }
+  // kPaged: the head's first page, its rows and 16-byte units from page to page
+  const char *kbase = reinterpret_cast<const char*>(a.kp.at(0, kvh, 0)), *vbase = reinterpret_cast<const char*>(a.vp.at(0, kvh, 0));
+  const uint32_t kps = static_cast<uint32_t>(a.kp.ps >> 3), vps = static_cast<uint32_t>(a.vp.ps >> 3);
   const uint32_t kfull = 7 * krs + 2 * a.dqk, vfull = 7 * vrs + 2 * a.dv;  // 8 rows
   auto load_tile = [&](int it, Index id, char* kt, char* vt) {
     const int j0 = k_begin + it * kKeys, left = k_end - j0;  // keys of the tile and behind
@@ -145,6 +155,15 @@ __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_ker
       }
       if (!ok) kr = vr = zeros;
       there = __ballot(ok);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 32 * i + 8 * wave;  // the load's first row
+        const char *kp = row_of(kr, r + lrow) + 2 * kdim, *vp = row_of(vr, r + lrow) + 2 * vdim;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) load_lds16(kdim + 64 * s < a.dqk ? kp + 128 * s : zeros, kt + r * 128 + s * P::PIECE);
+#pragma unroll
+        for (int s = 0; s < VS; ++s) load_lds16(vdim + 64 * s < a.dv ? vp + 128 * s : zeros, vt + r * 128 + s * P::PIECE);
+      }
     } else {
       there = left >= kKeys ? ~0ull : (1ull << left) - 1;
       if constexpr (SRC == kPaged) {
@@ -155,37 +174,35 @@ __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_ker
           there &= ~(0xffull << (8 * g));
         }
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 32 * i + 8 * wave;  // the load's first row
-      char* kd = kt + r * 128;
-      char* vd = vt + r * 128;
-      if constexpr (SRC == kAnywhere) {
-        const char *kp = row_of(kr, r + lrow) + 2 * kdim, *vp = row_of(vr, r + lrow) + 2 * vdim;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) load_lds16(kdim + 64 * s < a.dqk ? kp + 128 * s : zeros, kd + s * P::PIECE);
-#pragma unroll
-        for (int s = 0; s < VS; ++s) load_lds16(vdim + 64 * s < a.dv ? vp + 128 * s : zeros, vd + s * P::PIECE);
-      } else {
-        int n = min(8, max(0, left - r));  // its rows that exist
+      // the 8 rows from r on, of which n exist (scalar instructions, as many as the wave's vector ones: a whole tile skips
+      // what only the others need)
+      auto load_rows = [&](int i, int n, uint32_t kbytes, uint32_t vbytes) {
+        const int r = 32 * i + 8 * wave;
         const char *kb, *vb;
         if constexpr (SRC == kPaged) {
-          const int page = __builtin_amdgcn_readlane(static_cast<int>(id.lo), 4 * i + wave);
-          const int row = (j0 + r) - static_cast<int>(div_by(j0 + r, a.page)) * static_cast<int>(a.page.d);
-          if (!((there >> r) & 1)) n = 0;
-          kb = reinterpret_cast<const char*>(a.kp.at(n ? page : 0, kvh, row));
-          vb = reinterpret_cast<const char*>(a.vp.at(n ? page : 0, kvh, row));
+          const uint32_t page = n ? __builtin_amdgcn_readlane(id.lo, 4 * i + wave) : 0;
+          const uint32_t row = (j0 + r) - page_of(j0 + r) * a.page.d;
+          kb = kbase + (static_cast<uint64_t>(page) * kps << 4) + row * krs;
+          vb = vbase + (static_cast<uint64_t>(page) * vps << 4) + row * vrs;
         } else {
           kb = kpk + 32 * i * static_cast<int64_t>(krs);
           vb = vpk + 32 * i * static_cast<int64_t>(vrs);
         }
-        const uint32_t kbytes = n == 8 ? kfull : n ? (n - 1) * krs + 2 * a.dqk : 0, vbytes = n == 8 ? vfull : n ? (n - 1) * vrs + 2 * a.dv : 0;
         const rsrc_t kres = make_rsrc(kb, kbytes), vres = make_rsrc(vb, vbytes);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) buf_lds16(kres, kdim + 64 * s < a.dqk ? koff + 128u * s : kPast, kd + s * P::PIECE);
+        for (int s = 0; s < KS; ++s) buf_lds16(kres, kdim + 64 * s < a.dqk ? koff + 128u * s : kPast, kt + r * 128 + s * P::PIECE);
 #pragma unroll
-        for (int s = 0; s < VS; ++s) buf_lds16(vres, vdim + 64 * s < a.dv ? voff + 128u * s : kPast, vd + s * P::PIECE);
+        for (int s = 0; s < VS; ++s) buf_lds16(vres, vdim + 64 * s < a.dv ? voff + 128u * s : kPast, vt + r * 128 + s * P::PIECE);
+      };
+      if (there == ~0ull) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) load_rows(i, 8, kfull, vfull);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 32 * i + 8 * wave, n = (there >> r) & 1 ? min(8, left - r) : 0;
+          load_rows(i, n, n ? (n - 1) * krs + 2 * a.dqk : 0, n ? (n - 1) * vrs + 2 * a.dv : 0);
+        }
       }
     }
     if constexpr (SRC == kPacked) {
@@ -434,11 +451,15 @@ int launch_source(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const ch
 }
 
 // Packed rows, and pages of a multiple of 8 rows, are read 8 rows to an instruction through a resource that ends with them
-// (a resource reaches 2^31 bytes); other pages, and rows further apart, row by row from wherever they lie.
+// (a resource reaches 2^31 bytes, and addresses are counted in 32 bits: bytes within a page's head, 16-byte units from page
+// to page); other pages, and rows further apart, row by row from wherever they lie.
 template <class T>
 int launch_type(const AttnArgs& a, const AttnPlan& p, bool paged, hipStream_t st, const char* what) {
   const int64_t far = 1 << 26;  // elements between rows: 8 of them stay below 2^31 bytes
-  const bool near = paged ? a.page.d % 8 == 0 && a.kp.rs < far && a.vp.rs < far : a.k.ts < far && a.v.ts < far;
+  auto pool_near = [&](const Pool& x) {
+    return x.rs < far && static_cast<int64_t>(a.page.d) * x.rs < (1LL << 31) && (a.n_pages <= 1 || x.ps < (1LL << 35));
+  };
+  const bool near = paged ? a.page.d % 8 == 0 && pool_near(a.kp) && pool_near(a.vp) : a.k.ts < far && a.v.ts < far;
   if (!near) return launch_source<T, kAnywhere>(a, p, st, what);
   return paged ? launch_source<T, kPaged>(a, p, st, what) : launch_source<T, kPacked>(a, p, st, what);
 }
