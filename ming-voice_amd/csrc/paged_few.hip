@@ -427,7 +427,14 @@ int launch_shape(const AttnArgs& a, const AttnPlan& p, hipStream_t st, const cha
   if (rc || (rc = launch_index<P::BR, P::GR>(a, st, what))) return rc;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((p.blocks + p.target) * a.nkv)), dim3(NW * kWave), P::LDS, st, a);
   rc = mm::check_launch(what);
-  return rc || p.target == 0 ? rc : launch_join<T, P::BR, P::GR, 4, 4>(a, p, st, what);
+  if (rc || p.target == 0) return rc;
+  // Rows of the join: a workgroup takes four, each with 4 x 8 pieces a round (dv = 64), or where a block can have more than 32
+  // pieces one, with four times as many. us a call, four | one: one Talker stream behind 5000 positions 10.7 | 11.2, behind
+  // 20000 13.8 | 12.2, 120000 37 | 26; 16 / 2 heads of 256 behind 60000 109 | 66; 32 streams of 4 tokens of 32/8 heads of 128
+  // behind 8000 205 | 217.
+  const int64_t most = (PAGED ? a.batch.max_keys : a.batch.tokens) / P::GR;
+  return p.target > 32 * p.blocks && most > 32 ? launch_join<T, P::BR, P::GR, 1, 1>(a, p, st, what)
+                                               : launch_join<T, P::BR, P::GR, 4, 4>(a, p, st, what);
 }
 
 template <class T, bool PAGED>

@@ -185,7 +185,7 @@ def test_paged_attn(nh, nkv, dqk, dv, dtype, idx, page, layout, new, ctx, kind):
     check(got, s.oracle(), max(s.kv), dqk, dtype)
 
 
-@pytest.mark.parametrize("new,ctx", [([1], [5000]), ([1, 1, 1], [20000, 3, 0]), ([3, 1], [9000, 8191]), ([64], [6000]),
+@pytest.mark.parametrize("new,ctx", [([1], [5000]), ([1], [70000]), ([2, 1], [9, 40000]), ([1, 1, 1], [20000, 3, 0]), ([3, 1], [9000, 8191]), ([64], [6000]),
                                      ([200, 1, 17], [3000, 40, 2500]), ([700], [2000])])
 @pytest.mark.parametrize("nh,nkv,dqk,dv", [(14, 2, 64, 64), (4, 1, 128, 128), (2, 2, 192, 128), (4, 2, 256, 256)])
 def test_long_contexts(nh, nkv, dqk, dv, new, ctx):
