@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 
 // The same for blocks of many rows, which are cut into few pieces: dv / 4 lanes to a row, each through all pieces. Grid (cut
 // blocks, key / value heads, BR / ROWS) x 256. Bound by latency too: 8 us after pieces of 100 to 500 tokens of 32/8 heads
-// behind 611 to 5000 positions (79 us).
+// behind 611 to 5000 positions (75 us).
 template <class T, int BR, int GR, int ROWS>
 __global__ __launch_bounds__(256) void join_rows_kernel(AttnArgs a) {
   const int tid = threadIdx.x, kvh = blockIdx.y, G = static_cast<int>(a.group.d);

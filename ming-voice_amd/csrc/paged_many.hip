@@ -62,17 +62,18 @@ enum Source { kPacked, kPaged, kAnywhere };
 // requests its part of the next one (8 rows by 128 bytes an instruction). Swizzles keep every LDS read free of bank
 // conflicts (SQ_LDS_BANK_CONFLICT 0). All key fragments are read before the first product and all value fragments before
 // the softmax, so that neither waits for LDS.
-// Bound by how far matrix and vector work of the two workgroups of a CU overlap: at 8192 tokens of 32/8 heads of 128 (550
-// GFLOP of pairs that count) 549 us, 1.0 PFLOP/s, where the 8192^3 product runs at 1.15; the matrix units are busy 55 % of
-// the cycles, the vector units 50 %. At 64 dims the exponentials (a quarter of the vector rate) and 4 more vector
-// instructions a score weigh as much as the products twice: 12 Talker prompts of 5 to 2000 tokens 31.7 us (357 TFLOP/s),
-// 4000 tokens 52 us. On the way there (8192 tokens): 932 us with rows brought by ds_bpermute and fragments read one by one;
-// 673 with 64-dim pieces, one page to a load and the not-finite code out of the loop; 616 with the key fragments ahead, 588
-// with the value fragments too; 560 with one instruction to a pair of weights and to two of a maximum. Not kept: s_setprio
-// around the products (588 -> 600), exponentials dealt out between the products (627), for 256 dims the value fragments
-// ahead (spills); at 64 dims (2000 Talker tokens, 26.8 us) the last tile's value products under this tile's softmax (27.6),
-// the next tile's scores as well (33), tiles requested two ahead (28.2).
-
+// Bound at 128 dims by how far matrix and vector work of the two workgroups of a CU overlap: 8192 tokens of 32/8 heads (550
+// GFLOP of pairs that count) 549 us, 1.0 PFLOP/s, where the 8192^3 product runs at 1.15; the matrix units are busy 55 % of the
+// cycles, the vector units 50 %. At 64 dims by the issue of instructions, one a wave in four cycles whatever its kind, of which
+// the products are the least: 12 Talker prompts of 5 to 2000 tokens 32 us (353 TFLOP/s), 4000 tokens 50. So a tile's page
+// arithmetic is kept short (pieces of 100 to 500 tokens of 32/8 heads behind 611 to 5000 positions 85.6 -> 82.0 us on the GPU).
+// On the way there (8192 tokens): 932 us with rows brought by ds_bpermute and fragments read one by one; 673 with 64-dim
+// pieces, one page to a load and the not-finite code out of the loop; 616 with the key fragments ahead, 588 with the value
+// fragments too; 560 with one instruction to a pair of weights and to two of a maximum. Not kept: s_setprio around the
+// products (588 -> 600), exponentials dealt out between the products (627), for 256 dims the value fragments ahead (spills);
+// at 64 dims (2000 Talker tokens, 26.8 us) the last tile's value products under this tile's softmax (27.6), the next tile's
+// scores as well (33), tiles requested two ahead (28.2), or behind the scores (27.7), the weights summed by a matrix
+// instruction (27.1).
 template <class T, int KS, int VS, int NG, int SRC>
 __global__ __launch_bounds__(NG * kWaves * kWave, KS <= 3 ? 2 : 1) void many_kernel(AttnArgs a) {
   using P = Many<KS, VS, NG>;
