@@ -2,7 +2,8 @@
 // pages, and the attention over packed prompts (C ABI: mingpaged.h).
 //
 //   paged_append_kernel   rotation and stores, one pass over q, k and v
-//   few_kernel            attention of few rows, join_kernel (paged_few.hip)
+//   index_kernel          where each of many streams' work begins (paged_common.h)
+//   few_kernel            attention of few rows, and the joins of cut keys (paged_few.hip)
 //   many_kernel           attention of many rows (paged_many.hip)
 #include <cmath>
 

@@ -310,6 +310,21 @@ def test_offsets_past_32_bits():
     assert torch.equal(far_v.nan_to_num(7.0), s.vp.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("page,row", [(16, 1024), (56, 1 << 25), (64, 1 << 25)])
+def test_far_pages_in_a_block_of_many_rows(page, row):
+    """Pages 3 GiB apart, and rows of a page whose last lies before or past 2^32 bytes of its first."""
+    s = Streams([1, 20], [40, 3], nh=2, nkv=1, page=page, seed=31, more_pages=many_pages("many", page))
+    n, gap = s.kp.shape[0], max(3 << 29, page * row)
+    raw = torch.empty(n * gap, device=DEV, dtype=BF)
+    far = raw.as_strided(s.kp.shape, (gap, row, row, 1))
+    far_v = raw.as_strided(s.vp.shape, (gap, row, row, 1), 512)
+    far.copy_(s.kp)
+    far_v.copy_(s.vp)
+    got = PK.paged_attn(s.q, far, far_v, s.table, s.cu, s.lens)
+    assert torch.equal(got, s.attn())
+    check(got, s.oracle(), 64, 64, BF)
+
+
 def test_rows_far_apart_in_a_block_of_many_rows():
     """Keys and values 128 MiB apart, past what one buffer resource spans, at 512 query heads on one."""
     s = Streams([70, 30], [0, 0], nh=512, nkv=1, seed=30)
